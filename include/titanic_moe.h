@@ -88,6 +88,48 @@ int ca_ffn_sum_hc_post(void* context, int rows, int live, const void* routes, co
 int ca_ffn_sum_residual(void* context, int rows, int live, const void* routes, const void* shared, const void* residual, void* routed,
                         void* ffn_out, void* residual_out, void* stream);
 
+/* ---- a dense feed-forward block in MXFP4 ------------------------------------------------------------------------- */
+/* No counterpart in the reference, whose model has no dense feed-forward layer: the operators of a block
+ *   residual += x;  n = rmsnorm(residual);  h = swiglu(n . Up^T, n . Gate^T);  x = h . Down^T
+ * with MXFP4 weights (the experts' format: E2M1, blocks of 32 along the contraction, UE8M0 scales) and MXFP8 or MXFP4 activations.
+ * The context gives the MXFP8 block width (act_block) and the activation's clip (swiglu_limit); every other dimension is an
+ * argument.  All calls: rows 0 enqueues nothing and returns 0; -1 for a null or misaligned pointer, a size outside the
+ * ranges below, a stride shorter than its row, or a context opened on another device than the current one; nothing is
+ * allocated, kept from one call for the next, or waited for, so calls may overlap on any streams and be captured. */
+#define CA_TYPE_BF16 0
+#define CA_TYPE_FP16 1
+#define CA_TYPE_FP32 2
+#define CA_MX_E4M3 0      /* codes [rows][cols], scales [rows][cols / act_block] */
+#define CA_MX_E2M1 1      /* words [rows][cols / 2] (low nibble = even column), scales [rows][cols / 32] */
+/* r = bf16(x + residual) -> residual_out; normed = bf16((r / sqrt(mean(r^2) + eps)) * weight); the MXFP8 flavours of normed as
+ * ca_ffn_norm_quant gives them (codes: a zero block has scale byte 0; codes_min: amax floored at 1e-4).  Rows of x, residual and
+ * residual_out lie *_stride values apart (multiples of 8, pointers 16-byte aligned); normed, codes and scales are dense.  residual may
+ * be null (r = x), so may each output; residual_out may be residual or x.  cols: a multiple of act_block up to 8,192 (-4). */
+int ca_ffn_add_norm_quant(void* context, int rows, int cols, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                          const void* weight, float eps, void* residual_out, int64_t residual_out_stride, void* normed, void* codes, void* scales,
+                          void* codes_min, void* scales_min, void* stream);
+/* x [rows][cols] of CA_TYPE_* -> words and scales, in the canonical layout that ca_mxfp4_prepare and the expert preparation take.  A
+ * block's scale byte is floor(log2(amax)) - 2 + 127 within 1..247 (127 for a zero block), codes round to the nearest, ties to
+ * even, and saturate; a block that holds a NaN or an infinity has scale byte 255 and reads back as NaN.  cols: a multiple of 32;
+ * rows start at 16-byte boundaries; rows * cols < 2^34. */
+int ca_mxfp4_quant(void* context, int rows, int cols, const void* x, int64_t x_stride, int x_type, void* words, void* scales, void* stream);
+/* The values that words and scales stand for, rounded once to out_type. */
+int ca_mxfp4_dequant(void* context, int rows, int cols, const void* words, const void* scales, void* out, int64_t out_stride, int out_type, void* stream);
+/* Weights [n][k] from the canonical layout to the one that the products read (once, at load time; the layout of the layer's prepared
+ * experts, padded with zeros to whole tiles): bytes of the two destinations, and the copy.  n >= 1, k a multiple of 32 up to 65,536. */
+int64_t ca_mxfp4_words_bytes(int n, int k);
+int64_t ca_mxfp4_scales_bytes(int n, int k);
+int ca_mxfp4_prepare(void* context, int n, int k, const void* words, const void* scales, void* prepared_words, void* prepared_scales, void* stream);
+/* rows <= 4,194,304 in both products.  out[rows][n] (bf16, rows out_stride values apart) = a[rows][k] . w[n][k]^T.  a: codes or words of a_type (CA_MX_*), dense, 16-byte
+ * aligned; k a multiple of act_block for CA_MX_E4M3.  Sums are FP32 in the matrix core. */
+int ca_mxfp4_linear(void* context, int rows, int n, int k, const void* a, const void* a_scales, int a_type, const void* w, const void* w_scales, void* out,
+                    int64_t out_stride, void* stream);
+/* u = a . up^T, g = a . gate^T; act[rows][inter] = bf16(min(g, L) * logistic(min(g, L)) * clamp(u, -L, L)) with L = swiglu_limit; codes /
+ * scales: act quantized to out_type (CA_MX_*: MXFP8 in the context's blocks with scale byte 0 for a zero block, or MXFP4 as
+ * ca_mxfp4_quant).  act, or codes with scales, may be null.  inter: a multiple of the codes' block. */
+int ca_mxfp4_swiglu(void* context, int rows, int inter, int k, const void* a, const void* a_scales, int a_type, const void* up, const void* up_scales,
+                    const void* gate, const void* gate_scales, void* act, void* codes, void* scales, int out_type, void* stream);
+
 /* ---- kernels the reference resolves by name from a code module (src/cuda.rs:199-226 Module::function + launch) -- */
 /* Launches the `extern "C" __global__` kernel `name` with the reference's launch tuple ([grid;3], [block;3], dynamic
  * shared bytes, stream, argument pointers).  -3 for an unknown name.  The same kernels are in titanic_moe_gfx950.hsaco

@@ -8,6 +8,8 @@
 """
 import os
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -34,12 +36,25 @@ def _run(cmd):
     return lines
 
 
+# translation units of the kernel library: the MoE layer with the ABI, the dense feed-forward operators
+KERNEL_UNITS = ["abi.hip", "dense_ffn.hip"]
+
+
 def build_kernels():
-    src = os.path.join(CSRC, "abi.hip")
-    _run(["hipcc", *DEVICE_FLAGS, "-fPIC", "-shared", src, "-o", KERNEL_LIB])
-    _run(["hipcc", *DEVICE_FLAGS, "--genco", src, "-o", CODE_OBJECT])
-    # the kernels the reference launches by name with fixed argument lists, for its own layer's dimensions
-    _run(["hipcc", *DEVICE_FLAGS, "--genco", os.path.join(CSRC, "reference_layer.hip"), "-o", REFERENCE_LAYER_OBJECT])
+    def compile_unit(name, folder):
+        out = os.path.join(folder, name + ".o")
+        _run(["hipcc", *DEVICE_FLAGS, "-fPIC", "-c", os.path.join(CSRC, name), "-o", out])
+        return out
+
+    with tempfile.TemporaryDirectory() as folder, ThreadPoolExecutor(4) as pool:
+        units = [pool.submit(compile_unit, name, folder) for name in KERNEL_UNITS]
+        objects = [
+            pool.submit(_run, ["hipcc", *DEVICE_FLAGS, "--genco", os.path.join(CSRC, "abi.hip"), "-o", CODE_OBJECT]),
+            # the kernels the reference launches by name with fixed argument lists, for its own layer's dimensions
+            pool.submit(_run, ["hipcc", *DEVICE_FLAGS, "--genco", os.path.join(CSRC, "reference_layer.hip"), "-o", REFERENCE_LAYER_OBJECT])]
+        _run(["hipcc", "--offload-arch=gfx950", "-fPIC", "-shared", *[u.result() for u in units], "-o", KERNEL_LIB])
+        for o in objects:
+            o.result()
     return KERNEL_LIB
 
 

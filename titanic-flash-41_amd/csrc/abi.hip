@@ -1,6 +1,7 @@
 // C ABI of libtitanic_moe_hip.so: the entry points the reference's Rust FFN operators bind (see include/titanic_moe.h).
 // Nothing here allocates, frees or synchronizes; every entry point only enqueues kernels on the caller's stream.
 #include "../../include/titanic_moe.h"
+#include "context.hpp"
 #include "boundary.cuh"
 #include "codec.cuh"
 #include "combine.cuh"
@@ -40,19 +41,6 @@ int check_geometry(const ca_geometry& g) {
     return 0;
 }
 int launch_status() { return (int)hipGetLastError(); }
-
-struct Context {
-    ca_geometry g;
-    int cus;
-    int stream_wgs;    // persistent workgroups of the streaming kernels
-    hipEvent_t marks[7];   // profiling aid: see ca_primitives_marks
-    bool marking;
-    bool kernel_marks;     // marks[5], marks[6]: begin and end of the FC1 + SwiGLU kernel itself
-    int spin_limit;        // polls a wait inside the front-end launch may take before the waiter does the work itself
-    int shared_reserve;    // CUs the shared expert's many-row first projection leaves without a workgroup (0: none)
-    int device;            // the device the context was opened on
-    uint8_t* static_scratch;   // that device's copy of `scratch`
-};
 
 // The regions of entry 0 / 1's scratch arena, in the runtime contract's order, each aligned to 256 bytes: token codes and
 // scales (routed flavour, shared flavour), intermediate (BF16, codes, scales), tile tables, row maps, route outputs,

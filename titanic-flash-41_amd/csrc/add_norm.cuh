@@ -1,0 +1,104 @@
+// The boundary between two sublayers of a residual stream: the sublayer's output joins the residual, the sum is normalized and
+// quantized for the next product, in one pass over the row.
+//   r      = bf16(x + residual)                                       (residual == null: r = x)
+//   normed = bf16((r * (1 / sqrt(sum(r^2) / cols + eps))) * weight)     sum in FP32, division and root correctly rounded
+//   codes / scales (zero block: scale byte 0) and codes_min / scales_min (amax floored at 1e-4): the MXFP8 flavours of the normalized row,
+//   as ca_ffn_norm_quant has them
+// The statistics are those of the BF16 residual that the next boundary reads, so that they do not depend on who forms them.
+#pragma once
+#include "common.cuh"
+
+struct AddNormArgs {
+    const uint16_t *x, *residual, *weight;
+    uint16_t *residual_out, *normed;
+    uint8_t *codes, *scales, *codes_min, *scales_min;
+    long long x_stride, residual_stride, residual_out_stride;        // values
+    int rows, cols, act_block;
+    float eps;
+};
+
+// WAVES waves a row (1: four rows a workgroup; 4: one row a workgroup), PIECES 8-value pieces a lane.
+template <int WAVES, int PIECES>
+__global__ void __launch_bounds__(256) tf_add_norm_quant(const AddNormArgs p) {
+    constexpr int LANES = WAVES * 64;
+    __shared__ float s_wave[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int row = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= p.rows) return;                             // a whole wave (WAVES 1: no barrier below) or nobody
+    const int t = WAVES == 1 ? lane : threadIdx.x, per_row = p.cols >> 3, group_lanes = p.act_block >> 3;
+    const u4v* x = reinterpret_cast<const u4v*>(p.x + (long long)row * p.x_stride);
+    const u4v* res = reinterpret_cast<const u4v*>(p.residual + (long long)row * p.residual_stride);
+    u4v* res_out = reinterpret_cast<u4v*>(p.residual_out + (long long)row * p.residual_out_stride);
+    u4v r[PIECES];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int q = i * LANES + t;
+        r[i] = u4v{0, 0, 0, 0};
+        if (q < per_row) {
+            r[i] = x[q];
+            if (p.residual != nullptr) {
+                const u4v b = res[q];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    r[i][j] = tf_pack_bf16(__fadd_rn(tf_bf16_lo(r[i][j]), tf_bf16_lo(b[j])), __fadd_rn(tf_bf16_hi(r[i][j]), tf_bf16_hi(b[j])));
+            }
+            if (p.residual_out != nullptr) res_out[q] = r[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            ss = __fmaf_rn(tf_bf16_lo(r[i][j]), tf_bf16_lo(r[i][j]), ss);
+            ss = __fmaf_rn(tf_bf16_hi(r[i][j]), tf_bf16_hi(r[i][j]), ss);
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) ss = __fadd_rn(ss, __shfl_xor(ss, o));
+    if constexpr (WAVES > 1) {
+        if (lane == 0) s_wave[wave] = ss;
+        __syncthreads();
+        ss = __fadd_rn(__fadd_rn(__fadd_rn(s_wave[0], s_wave[1]), s_wave[2]), s_wave[3]);
+    }
+    const float inverse = 1.0f / __builtin_sqrtf(__fadd_rn(ss / (float)p.cols, p.eps));
+    const u4v* weight = reinterpret_cast<const u4v*>(p.weight);
+    const int groups = p.cols / p.act_block;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int q = i * LANES + t;
+        const bool on = q < per_row;                       // whole groups of lanes together: per_row is a multiple of group_lanes
+        float v[8];
+        u4v o = {0, 0, 0, 0};
+        if (on) {
+            const u4v w = weight[q];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                o[j] = tf_pack_bf16(__fmul_rn(__fmul_rn(tf_bf16_lo(r[i][j]), inverse), tf_bf16_lo(w[j])),
+                                    __fmul_rn(__fmul_rn(tf_bf16_hi(r[i][j]), inverse), tf_bf16_hi(w[j])));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[2 * j] = tf_bf16_lo(o[j]); v[2 * j + 1] = tf_bf16_hi(o[j]); }
+        const float amax = tf_group_amax(v, group_lanes);
+        if (!on) continue;
+        const size_t at = (size_t)row * per_row + q;
+        const size_t group = (size_t)row * groups + q / group_lanes;
+        if (p.normed != nullptr) reinterpret_cast<u4v*>(p.normed)[at] = o;
+        if (p.codes != nullptr) {
+            const Quant8 c = tf_quant8(v, amax, 0.f);
+            reinterpret_cast<u2v*>(p.codes)[at] = u2v{c.lo, c.hi};
+            if ((q & (group_lanes - 1)) == 0) p.scales[group] = (uint8_t)c.exponent;
+        }
+        if (p.codes_min != nullptr) {
+            const Quant8 c = tf_quant8(v, amax, 1e-4f);
+            reinterpret_cast<u2v*>(p.codes_min)[at] = u2v{c.lo, c.hi};
+            if ((q & (group_lanes - 1)) == 0) p.scales_min[group] = (uint8_t)c.exponent;
+        }
+    }
+}
+// One wave a row up to 2,048 columns (four pieces a lane, no exchange between waves), four waves beyond.
+inline void tf_launch_add_norm(const AddNormArgs& p, hipStream_t s) {
+    const int grid = p.cols <= 2048 ? (p.rows + 3) / 4 : p.rows;
+    if (p.cols <= 512) tf_add_norm_quant<1, 1><<<grid, 256, 0, s>>>(p);
+    else if (p.cols <= 1024) tf_add_norm_quant<1, 2><<<grid, 256, 0, s>>>(p);
+    else if (p.cols <= 2048) tf_add_norm_quant<1, 4><<<grid, 256, 0, s>>>(p);
+    else if (p.cols <= 4096) tf_add_norm_quant<4, 2><<<grid, 256, 0, s>>>(p);
+    else tf_add_norm_quant<4, 4><<<grid, 256, 0, s>>>(p);
+}

@@ -16,7 +16,13 @@ EXPORTS = ["ca_ffn_abi", "ca_ffn_configure", "ca_ffn_geometry", "ca_router_logit
            "ca_primitives_entries", "ca_primitives_scratch_bytes", "ca_primitives_marks", "ca_encode", "ca_decode", "ca_local_live",
            "ca_pack_bf16", "ca_primitives_spin_limit", "ca_primitives_shared_reserve", "ca_primitives_open_geometry", "ca_primitives_geometry", "ca_router_logits_in",
            "ca_router_logits_wide_in", "ca_shared_swiglu_in", "ca_ffn_add_in", "ca_moe_dynamic_static", "ca_moe_dynamic_static_capacity",
-           "ca_ffn_norm_quant", "ca_ffn_sum_residual", "ca_hc_combine_norm_quant", "ca_hc_post", "ca_ffn_sum_hc_post"]
+           "ca_ffn_norm_quant", "ca_ffn_sum_residual", "ca_hc_combine_norm_quant", "ca_hc_post", "ca_ffn_sum_hc_post",
+           "ca_ffn_add_norm_quant", "ca_mxfp4_quant", "ca_mxfp4_dequant", "ca_mxfp4_words_bytes", "ca_mxfp4_scales_bytes", "ca_mxfp4_prepare",
+           "ca_mxfp4_linear", "ca_mxfp4_swiglu"]
+
+# ca_mxfp4_*: element types of plain tensors, number formats of quantized ones
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
+MX_E4M3, MX_E2M1 = 0, 1
 
 
 class Geometry(ctypes.Structure):
@@ -95,6 +101,16 @@ def load():
     lib.ca_hc_combine_norm_quant.argtypes = [vp, ctypes.c_int, ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.ca_hc_post.argtypes = [vp, ctypes.c_int, vp, vp, vp, vp, vp, vp]
     lib.ca_ffn_sum_hc_post.argtypes = [vp, ctypes.c_int, ctypes.c_int, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    i64, ci = ctypes.c_int64, ctypes.c_int
+    lib.ca_ffn_add_norm_quant.argtypes = [vp, ci, ci, vp, i64, vp, i64, vp, ctypes.c_float, vp, i64, vp, vp, vp, vp, vp, vp]
+    lib.ca_mxfp4_quant.argtypes = [vp, ci, ci, vp, i64, ci, vp, vp, vp]
+    lib.ca_mxfp4_dequant.argtypes = [vp, ci, ci, vp, vp, vp, i64, ci, vp]
+    for name in ("ca_mxfp4_words_bytes", "ca_mxfp4_scales_bytes"):
+        getattr(lib, name).restype = i64
+        getattr(lib, name).argtypes = [ci, ci]
+    lib.ca_mxfp4_prepare.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
+    lib.ca_mxfp4_linear.argtypes = [vp, ci, ci, ci, vp, vp, ci, vp, vp, vp, i64, vp]
+    lib.ca_mxfp4_swiglu.argtypes = [vp, ci, ci, ci, vp, vp, ci, vp, vp, vp, vp, vp, vp, vp, ci, vp]
     _lib = lib
     return lib
 
