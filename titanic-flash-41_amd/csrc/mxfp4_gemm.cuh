@@ -15,14 +15,21 @@
 // prepared, 1 KiB a 16-row tile and k-step in fragment order.  Scales come once a round of four k-steps, a byte of a register a k-step.
 #pragma once
 #include "mxfp4_stream.cuh"
+#include <utility>
 
-// Lane l of the wave copies 16 (4) bytes from global address base + offset to LDS byte address lds_base + 16 l (4 l).
-__device__ __forceinline__ void tf_mx_dma16(const uint8_t* base, uint32_t offset, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds_base) : "memory", "m0");
+// Requests: lane l copies 16 (4) bytes from its address to LDS byte address m0 + OFFSET + 16 l (4 l); OFFSET is added to the memory
+// address too.  m0 is set apart from them, once for several requests, and nothing else in the kernel writes it.
+__device__ __forceinline__ void tf_mx_m0(uint32_t lds_base) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0" ::"s"(lds_base) : "memory"); }
+template <int OFFSET>
+__device__ __forceinline__ void tf_mx_dma16(const uint8_t* base, uint32_t offset) {
+    asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" ::"v"(offset), "s"(base), "n"(OFFSET) : "memory");
 }
-__device__ __forceinline__ void tf_mx_dma4(const uint8_t* base, uint32_t offset, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(lds_base) : "memory", "m0");
-}
+__device__ __forceinline__ void tf_mx_dma16(const uint8_t* from) { asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(from) : "memory"); }
+__device__ __forceinline__ void tf_mx_dma4(const uint8_t* from) { asm volatile("global_load_lds_dword %0, off" ::"v"(from) : "memory"); }
+template <class F, int... I>
+__device__ __forceinline__ void tf_static_for(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void tf_static_for(F&& f) { tf_static_for(f, std::make_integer_sequence<int, N>{}); }
 template <int N>
 __device__ __forceinline__ void tf_mx_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void tf_mx_barrier() {                  // LDS accesses done, then everyone's
@@ -92,14 +99,18 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
 
     // ---- requests ----------------------------------------------------------------------------------------------------
     const uint32_t lds_ring = tf_mx_lds(s_ring), lds_wsc = tf_mx_lds(s_wsc), lds_asc = tf_mx_lds(s_asc);
-    const uint8_t* a_base = p.a + (size_t)row0 * a_pitch;
-    uint32_t a_row[NA], a_col[NA];
+    // Every request is a scalar base that moves on with the k-step plus the lane's own offset; four requests share an m0, so a request's
+    // offset holds 1,024 bytes for every one before it in its four less (and the bases point 4,096 bytes before their data).
+    constexpr bool WHOLE = SC != MX_SCALES_ANY;                              // k is whole rounds: no request needs a bound
+    const uint8_t* a_base = p.a + (size_t)row0 * a_pitch - 4096;
+    uint32_t a_off[NA], a_col[NA];
 #pragma unroll
     for (int c = 0; c < NA; ++c) {
         const int row = (wave * NA + c) * ROWS_REQ + lane / LANES_ROW, r = row & 15;
         const int swz = FP4A ? ((r >> 1) & 3) ^ (r >> 3) : (r & 7) ^ (r >> 3);
-        a_row[c] = (uint32_t)min(row, rows - 1) * (uint32_t)a_pitch;        // past the last row: that row again, never stored
         a_col[c] = (uint32_t)((lane % LANES_ROW) ^ swz) * 16;
+        // past the last row: that row again, never stored
+        a_off[c] = (uint32_t)min(row, rows - 1) * (uint32_t)a_pitch + 4096 - 1024 * (c & 3) + (WHOLE ? a_col[c] : 0);
     }
     // weight tile T of the workgroup (gated: a wave's FT tiles are FT / 2 of `up`, then the same columns' of `gate`)
     auto weight_tile = [&](int T, bool& second) {
@@ -108,12 +119,17 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
         const int tile = GATED ? tile_n * (TILES / 2) + w * (FT / 2) + (second ? t - FT / 2 : t) : tile_n * TILES + T;
         return min(tile, n_tiles - 1);                                       // past the last tile: that tile again, never stored
     };
-    const uint8_t* b_base[NB];
-#pragma unroll
-    for (int c = 0; c < NB; ++c) {
+    // the tiles a wave requests are all of one matrix (NB <= FT / 2)
+    static_assert(!GATED || FT / 2 % NB == 0, "one matrix a wave's requests");
+    const uint32_t lane16 = lane * 16;
+    const uint8_t* b_base;
+    uint32_t b_off[NB];
+    {
         bool second;
-        const int tile = weight_tile(wave * NB + c, second);
-        b_base[c] = reinterpret_cast<const uint8_t*>(second ? p.w2 : p.w) + (size_t)tile * KS * 1024;
+        const int first = weight_tile(wave * NB, second);
+        b_base = reinterpret_cast<const uint8_t*>(second ? p.w2 : p.w) + (size_t)first * KS * 1024 - 4096;
+#pragma unroll
+        for (int c = 0; c < NB; ++c) b_off[c] = (uint32_t)(weight_tile(wave * NB + c, second) - first) * (uint32_t)KS * 1024 + lane16 + 4096 - 1024 * (c & 3);
     }
     // weight scales: a wave requests four tiles' 256 bytes of the round at once, 16 lanes a tile
     const uint8_t* wsc_base;
@@ -123,24 +139,28 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
         wsc_base = reinterpret_cast<const uint8_t*>(second ? p.ws2 : p.ws) + (size_t)tile * KQ * 256 + (lane & 15) * 16;
     }
     const uint8_t* asc_row = p.a_scales + (size_t)(row0 + min(tid & (BM - 1), rows - 1)) * s_pitch;
-    const uint8_t* zeros = reinterpret_cast<const uint8_t*>(tf_mx_zeros);
-    const uint32_t lane16 = lane * 16;
-    auto issue = [&](int op, int ks, int stage) {                            // request `op` of k-step ks into ring stage `stage`
-        if (op < NA) tf_mx_dma16(a_base, a_row[op] + min((uint32_t)ks * ROWB + a_col[op], (uint32_t)a_pitch - 16), lds_ring + stage * STAGE + (wave * NA + op) * 1024);
-        else tf_mx_dma16(ks < KS ? b_base[op - NA] + (size_t)ks * 1024 : zeros, lane16, lds_ring + stage * STAGE + A_STAGE + (wave * NB + op - NA) * 1024);
-    };
-    auto copy16 = [&](const uint8_t* from, uint32_t lds) {                   // a lane's own 64-bit address
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
-    };
-    auto copy4 = [&](const uint8_t* from, uint32_t lds) {
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
+    const uint8_t* zeros = reinterpret_cast<const uint8_t*>(tf_mx_zeros) - 4096;
+    // Request OP of k-step ks into the ring stage at lds_stage; the first of four sets m0.
+    auto issue = [&](auto op_constant, int ks, uint32_t lds_stage) {
+        constexpr int OP = decltype(op_constant)::value;
+        if constexpr (OP < NA) {
+            if constexpr (OP % 4 == 0) tf_mx_m0(lds_stage + (wave * NA + OP) * 1024);
+            if constexpr (WHOLE) tf_mx_dma16<1024 * (OP & 3)>(a_base + (size_t)ks * ROWB, a_off[OP]);
+            else tf_mx_dma16<1024 * (OP & 3)>(a_base, a_off[OP] + min((uint32_t)ks * ROWB + a_col[OP], (uint32_t)a_pitch - 16));
+        } else {
+            constexpr int C = OP - NA;
+            if constexpr (C % 4 == 0) tf_mx_m0(lds_stage + A_STAGE + (wave * NB + C) * 1024);
+            if constexpr (WHOLE) tf_mx_dma16<1024 * (C & 3)>(b_base + (size_t)ks * 1024, b_off[C]);
+            else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? b_base + (size_t)ks * 1024 : zeros, ks < KS ? b_off[C] : lane16 + 4096 - 1024 * (C & 3));
+        }
     };
     const int asc_wave = wave & (BM / 64 - 1);                               // waves past the tile's rows repeat the first ones' request
     auto issue_scales = [&](int kq) {                                        // the MORE requests of a round (kq clamped: the count stays)
         kq = min(kq, KQ - 1);
-        copy16(wsc_base + (size_t)kq * 256, lds_wsc + wave * 1024);
-        if constexpr (SC == MX_SCALES_32) copy16(asc_row + kq * 16, lds_asc + asc_wave * 1024);
-        if constexpr (SC == MX_SCALES_128) copy4(asc_row + kq * 4, lds_asc + asc_wave * 256);
+        tf_mx_m0(lds_wsc + wave * 1024);
+        tf_mx_dma16(wsc_base + (size_t)kq * 256);
+        if constexpr (SC == MX_SCALES_32) { tf_mx_m0(lds_asc + asc_wave * 1024); tf_mx_dma16(asc_row + kq * 16); }
+        if constexpr (SC == MX_SCALES_128) { tf_mx_m0(lds_asc + asc_wave * 256); tf_mx_dma4(asc_row + kq * 4); }
     };
     uint32_t any[16];
     auto read_scales = [&](int kq) {                                         // MX_SCALES_ANY: this thread's row, one byte a block of 32
@@ -190,9 +210,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
     if constexpr (SC == MX_SCALES_ANY) { read_scales(0); write_scales(); }
     issue_scales(0);
 #pragma unroll
-    for (int d = 0; d < NS; ++d)
-#pragma unroll
-        for (int op = 0; op < DATA; ++op) issue(op, d, d);
+    for (int d = 0; d < NS; ++d) tf_static_for<DATA>([&](auto op) { issue(op, d, lds_ring + d * STAGE); });
     tf_mx_wait<(NS - 1) * DATA>();
     tf_mx_barrier();
 #pragma unroll
@@ -218,23 +236,25 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
         }
         if constexpr (Q == 2 && SC == MX_SCALES_ANY) write_scales();
         const int ahead = min(ks + NS, 4 * KQ - 1);                          // behind the last: that one again, never read
-#pragma unroll
-        for (int f = 0; f < FM; ++f) {
-            // fragment f's products, beside them what the next k-step needs from LDS and a share of the requests
-            read_a(av[Y][f], f, next);
-#pragma unroll
-            for (int t = f * FT / FM; t < (f + 1) * FT / FM; ++t) read_w(wv[Y][t], t, next);
-            if constexpr (Q == 3) {
-                read_sa(sa[1][f], f);
-#pragma unroll
-                for (int t = f * FT / FM; t < (f + 1) * FT / FM; ++t) read_sw(sw[1][t], t);
+        const uint32_t lds_now = lds_ring + now * STAGE;
+        // Product i (fragment i / FT, tile i % FT); behind it, spread over the step, what the next k-step needs from LDS (weights first) and the
+        // requests, one instruction between two products where it fits: the wave is alone on its SIMD, and what does not issue under a
+        // product leaves the matrix pipeline idle.
+        constexpr int P = FM * FT, READS = FT + FM, SCALES = Q == 3 ? FT + FM : 0, ALL = READS + SCALES;
+        tf_static_for<P>([&](auto i_constant) {
+            constexpr int I = decltype(i_constant)::value, F = I / FT, T = I % FT;
+            tf_mx_mfma<Q, Q>(acc[F][T], wv[X][T], av[X][F], sw[0][T], sa[0][F]);
+            constexpr int R = I * ALL * 4 / (P * 3), R_NEXT = (I + 1) * ALL * 4 / (P * 3);       // within the first three quarters
+            if constexpr (R_NEXT > R && R < ALL) {
+                if constexpr (R < FT) read_w(wv[Y][R], R, next);
+                else if constexpr (R < READS) read_a(av[Y][R - FT], R - FT, next);
+                else if constexpr (R < READS + FT) read_sw(sw[1][R - READS], R - READS);
+                else read_sa(sa[1][R - READS - FT], R - READS - FT);
             }
-#pragma unroll
-            for (int t = 0; t < FT; ++t) tf_mx_mfma<Q, Q>(acc[f][t], wv[X][t], av[X][f], sw[0][t], sa[0][f]);
-#pragma unroll
-            for (int op = f * DATA / FM; op < (f + 1) * DATA / FM; ++op) issue(op, ahead, now);
+            constexpr int D = I * DATA / P, D_LAST = I == 0 ? -1 : (I - 1) * DATA / P;
+            if constexpr (D != D_LAST) issue(std::integral_constant<int, D>{}, ahead, lds_now);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
         stage = next;
     };
     for (int kq = 0; kq < KQ; ++kq) {
@@ -250,33 +270,39 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
     tf_mx_wait<0>();                                                         // nothing writes LDS any more
     tf_mx_settle(acc);
 
-    // ---- results: lane (g, r16) of acc[f][t] holds columns 4 g .. 4 g + 3 of tile t for token row 16 f + r16 of the wave -----------
-    const int first_row = wm * 16 * FM + r16;
+    // ---- results ---------------------------------------------------------------------------------------------------------
+    // Lane (g, r16) of acc[f][t] holds columns 4 g .. 4 g + 3 of tile t for token row 16 f + r16 of the wave.  They pass through LDS as BF16 rows of
+    // 256 bytes (eight-byte chunks permuted by the row: a row's own lanes would all meet in four banks), so that what follows is one short
+    // loop over whole 16-byte pieces of rows: written out for every accumulator, its code alone was 50 KiB and ran at the speed of
+    // the instruction cache's misses (17 us a tile).
+    tf_mx_barrier();                                                         // every wave has read its last stage
     if constexpr (!GATED) {
+        constexpr int RB = FT * 32, PIECES = RB / 16;                        // a wave's own rows of 16 FT columns
+        uint8_t* own = s_ring + wave * (16 * FM * RB);
+        static_assert(RB == 256 && WAVES * 16 * FM * RB <= NS * STAGE, "rows of 32 chunks");
 #pragma unroll
-        for (int f = 0; f < FM; ++f) {
-            const int row = first_row + 16 * f;
-            __builtin_amdgcn_sched_barrier(0);
-            if (row < rows) {
-                uint16_t* to = p.out + (size_t)(row0 + row) * p.out_stride;
+        for (int f = 0; f < FM; ++f)
 #pragma unroll
-                for (int t = 0; t < FT; ++t) {
-                    const int col = tile_n * COLS + (wn * FT + t) * 16 + 4 * g;
-                    const u2v o = {tf_pack_bf16(acc[f][t][0], acc[f][t][1]), tf_pack_bf16(acc[f][t][2], acc[f][t][3])};
-                    if (p.wide && col + 4 <= p.n) *reinterpret_cast<u2v*>(to + col) = o;
-                    else
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) if (col + j < p.n) to[col + j] = (uint16_t)(o[j >> 1] >> (16 * (j & 1)));
+            for (int t = 0; t < FT; ++t)
+                *reinterpret_cast<u2v*>(own + (16 * f + r16) * RB + (((t * 4 + g) ^ (r16 << 1)) << 3)) =
+                    u2v{tf_pack_bf16(acc[f][t][0], acc[f][t][1]), tf_pack_bf16(acc[f][t][2], acc[f][t][3])};
+        const int piece = lane % PIECES, col = tile_n * COLS + wn * FT * 16 + piece * 8;
+#pragma unroll 4
+        for (int r = lane / PIECES; r < 16 * FM; r += 64 / PIECES) {
+            const u4v o = *reinterpret_cast<const u4v*>(own + r * RB + (((piece << 1) ^ ((r & 15) << 1)) << 3));
+            const int row = wm * 16 * FM + r;
+            if (row < rows && col < p.n) {
+                uint16_t* to = p.out + (size_t)(row0 + row) * p.out_stride + col;
+                if (p.wide == 2 && col + 8 <= p.n) *reinterpret_cast<u4v*>(to) = o;
+                else {
+                    const int count = min(8, p.n - col);
+                    for (int j = 0; j < count; ++j) to[j] = (uint16_t)(o[j >> 1] >> (16 * (j & 1)));
                 }
             }
         }
     } else {
-        constexpr int HT = FT / 2;                                           // activation tiles of the wave
-        static_assert(HT % 2 == 0, "whole blocks of 32 columns a wave");
-        float* s_max = reinterpret_cast<float*>(s_ring);                     // [WN][BM]: row maxima of the waves' columns (blocks of 128)
-        tf_mx_barrier();                                                     // every wave has read its last stage
-        u2v h[FM][HT];
-        float amax[FM][HT / 2];
+        constexpr int HT = FT / 2, RB = COLS * 2, PIECES = RB / 16;          // the workgroup's rows of COLS columns of the activation
+        static_assert(RB == 256 && BM * RB <= NS * STAGE, "rows of 32 chunks");
 #pragma unroll
         for (int f = 0; f < FM; ++f) {
             __builtin_amdgcn_sched_barrier(0);
@@ -285,72 +311,15 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
                 float v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = tf_mx_swiglu(acc[f][t][i], acc[f][HT + t][i], p.limit);
-                h[f][t] = u2v{tf_pack_bf16(v[0], v[1]), tf_pack_bf16(v[2], v[3])};
-            }
-#pragma unroll
-            for (int b = 0; b < HT / 2; ++b) {
-                // bits of the magnitudes: a NaN orders above everything (E2M1); the E4M3 scale leaves NaNs out, as the row quantizers do
-                uint32_t m = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t w = h[f][2 * b + (j >> 1)][j & 1], lo = w & 0x7fffu, hi = (w >> 16) & 0x7fffu;
-                    m = max(m, p.out_fp4 || lo <= 0x7f80u ? lo : 0u);
-                    m = max(m, p.out_fp4 || hi <= 0x7f80u ? hi : 0u);
-                }
-                m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-                m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-                amax[f][b] = __uint_as_float(m << 16);
+                *reinterpret_cast<u2v*>(s_ring + (wm * 16 * FM + 16 * f + r16) * RB + ((((wn * HT + t) * 4 + g) ^ (r16 << 1)) << 3)) =
+                    u2v{tf_pack_bf16(v[0], v[1]), tf_pack_bf16(v[2], v[3])};
             }
         }
-        if (p.codes != nullptr && p.out_block == 128) {                      // the 128 columns lie in WN / (COLS / 128) waves
-            constexpr int SHARE = 128 / (HT * 16);                           // waves a block
-#pragma unroll
-            for (int f = 0; f < FM; ++f) {
-                float m = amax[f][0];
-#pragma unroll
-                for (int b = 1; b < HT / 2; ++b) m = fmaxf(m, amax[f][b]);
-                if (g == 0) s_max[wn * BM + first_row + 16 * f] = m;
-            }
-            tf_mx_barrier();
-#pragma unroll
-            for (int f = 0; f < FM; ++f) {
-                float m = 0.f;
-#pragma unroll
-                for (int i = 0; i < SHARE; ++i) m = fmaxf(m, s_max[(wn / SHARE * SHARE + i) * BM + first_row + 16 * f]);
-#pragma unroll
-                for (int b = 0; b < HT / 2; ++b) amax[f][b] = m;
-            }
-        }
-#pragma unroll
-        for (int f = 0; f < FM; ++f) {
-            const int row = first_row + 16 * f;
-            if (row >= rows) continue;
-            const size_t at = (size_t)(row0 + row);
-#pragma unroll
-            for (int b = 0; b < HT / 2; ++b) {
-                const int block_col = tile_n * COLS + wn * HT * 16 + b * 32;
-                if (block_col >= p.n) continue;                              // n is a multiple of 32
-                const uint32_t bits = __float_as_uint(amax[f][b]);
-                const uint32_t e = p.out_fp4 ? tf_mxfp4_scale(bits) : tf_block_exponent(amax[f][b]);
-                const float inverse = p.out_fp4 ? tf_mxfp4_inverse(bits, e) : tf_block_inverse(e);
-#pragma unroll
-                for (int t = 2 * b; t < 2 * b + 2; ++t) {
-                    const int col = block_col + (t - 2 * b) * 16 + 4 * g;
-                    if (p.act != nullptr) *reinterpret_cast<u2v*>(p.act + at * p.n + col) = h[f][t];
-                    if (p.codes != nullptr) {
-                        const float v[4] = {tf_bf16_lo(h[f][t][0]), tf_bf16_hi(h[f][t][0]), tf_bf16_lo(h[f][t][1]), tf_bf16_hi(h[f][t][1])};
-                        if (p.out_fp4) {
-                            const float v8[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
-                            *reinterpret_cast<uint16_t*>(p.codes + at * (p.n >> 1) + (col >> 1)) = (uint16_t)tf_mxfp4_codes8(v8, inverse);
-                        } else {
-                            *reinterpret_cast<uint32_t*>(p.codes + at * p.n + col) =
-                                tf_pack_e4m3(__fmul_rn(v[0], inverse), __fmul_rn(v[1], inverse), __fmul_rn(v[2], inverse), __fmul_rn(v[3], inverse));
-                        }
-                    }
-                }
-                if (p.codes != nullptr && g == 0 && (p.out_block == 32 || (block_col & 127) == 0))
-                    p.scales[at * (p.n / p.out_block) + block_col / p.out_block] = (uint8_t)e;
-            }
+        tf_mx_barrier();
+        const int piece = lane % PIECES, col = tile_n * COLS + piece * 8;
+        for (int r = tid / PIECES; r < BM; r += WAVES * 64 / PIECES) {
+            const u4v h = *reinterpret_cast<const u4v*>(s_ring + r * RB + (((piece << 1) ^ ((r & 15) << 1)) << 3));
+            tf_mx_store_activation(p, h, (size_t)(row0 + r), col, r < rows && col < p.n);
         }
     }
 }

@@ -16,7 +16,7 @@ struct MxArgs {
     // product
     uint16_t* out;
     long long out_stride;
-    int wide;                            // whole 8-byte stores of a row's column quads are aligned
+    int wide;                            // stores of 8 bytes (1) or of 16 too (2) to a row's multiples of four (eight) columns are aligned
     // gated product
     uint16_t* act;
     uint8_t *codes, *scales;
@@ -49,14 +49,12 @@ __device__ __forceinline__ float tf_mx_swiglu(float up, float gate, float limit)
     const float u = up > limit ? limit : up < -limit ? -limit : up;
     return __fmul_rn(__fmul_rn(g, tf_logistic_fast(g)), u);
 }
-// Eight consecutive columns of the activation, rounded to BF16, per lane: the BF16 copy, the codes and the block's scale byte.  All lanes of
+// Eight consecutive columns of the activation (BF16) per lane: the BF16 copy, the codes and the block's scale byte.  All lanes of
 // the wave call; `on`: the lane's columns exist.  Adjacent lanes hold adjacent columns, a block's lanes start at a multiple of their count.
-__device__ __forceinline__ void tf_mx_store_activation(const MxArgs& p, const float (&h)[8], size_t row, int col, bool on) {
-    u4v o;
+__device__ __forceinline__ void tf_mx_store_activation(const MxArgs& p, const u4v& o, size_t row, int col, bool on) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        o[j] = tf_pack_bf16(h[2 * j], h[2 * j + 1]);
         v[2 * j] = tf_bf16_lo(o[j]);
         v[2 * j + 1] = tf_bf16_hi(o[j]);
     }
@@ -178,9 +176,10 @@ __global__ void __launch_bounds__(NW == 1 ? 512 : 1024) tf_mx_stream(const MxArg
             constexpr int PIECES = COLS / 8;
             for (int i = threadIdx.x; i < 16 * PIECES; i += blockDim.x) {
                 const int r = i / PIECES, piece = i % PIECES, at = row0 + 16 * m + r, col = blockIdx.x * COLS + piece * 8;
-                float h[8];
+                const float* from = s_h + r * (COLS + 4) + piece * 8;
+                u4v h;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = s_h[r * (COLS + 4) + piece * 8 + j];
+                for (int j = 0; j < 4; ++j) h[j] = tf_pack_bf16(from[2 * j], from[2 * j + 1]);
                 tf_mx_store_activation(p, h, (size_t)at, col, at < p.rows && col < p.n);
             }
         }
