@@ -72,12 +72,12 @@ enum { MX_SCALES_32 = 0,      // blocks of 32, k a multiple of 512: 16 bytes a r
 static __device__ const u4v tf_mx_zeros[64] = {};
 
 template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
-__global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 16 ? 2 : 3) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
     constexpr int WAVES = WM * WN, BM = 16 * FM * WM, TILES = FT * WN, ROWB = FP4A ? 64 : 128;
     constexpr int A_STAGE = BM * ROWB, B_STAGE = TILES * 1024, STAGE = A_STAGE + B_STAGE;
     constexpr int NA = A_STAGE / 1024 / WAVES, NB = TILES / WAVES, DATA = NA + NB, MORE = SC == MX_SCALES_ANY ? 1 : 2;
     constexpr int COLS = (GATED ? TILES / 2 : TILES) * 16, LANES_ROW = ROWB / 16, ROWS_REQ = 64 / LANES_ROW;
-    static_assert(NA * WAVES * 1024 == A_STAGE && NB * WAVES == TILES && TILES == 4 * WAVES && BM <= WAVES * 64 && (SC != MX_SCALES_ANY || BM == WAVES * 64), "whole requests a wave");
+    static_assert(NA * WAVES * 1024 == A_STAGE && NB * WAVES == TILES && TILES % 4 == 0 && TILES <= 4 * WAVES && BM % 64 == 0 && BM <= WAVES * 64, "whole requests a wave");
     typedef typename MxFragment<FP4A>::type Fragment;
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NS * STAGE];
     __shared__ __attribute__((aligned(1024))) uint32_t s_wsc[TILES * 64];
@@ -119,23 +119,27 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
         const int tile = GATED ? tile_n * (TILES / 2) + w * (FT / 2) + (second ? t - FT / 2 : t) : tile_n * TILES + T;
         return min(tile, n_tiles - 1);                                       // past the last tile: that tile again, never stored
     };
-    // the tiles a wave requests are all of one matrix (NB <= FT / 2)
-    static_assert(!GATED || FT / 2 % NB == 0, "one matrix a wave's requests");
+    // the tiles a wave requests are of one matrix (gated: NB <= FT / 2), or half of them of either (NB == FT)
+    constexpr bool BOTH = GATED && NB == FT;
+    static_assert(!GATED || BOTH || FT / 2 % NB == 0, "whole halves");
     const uint32_t lane16 = lane * 16;
-    const uint8_t* b_base;
+    const uint8_t* b_base[2];
     uint32_t b_off[NB];
-    {
-        bool second;
-        const int first = weight_tile(wave * NB, second);
-        b_base = reinterpret_cast<const uint8_t*>(second ? p.w2 : p.w) + (size_t)first * KS * 1024 - 4096;
 #pragma unroll
-        for (int c = 0; c < NB; ++c) b_off[c] = (uint32_t)(weight_tile(wave * NB + c, second) - first) * (uint32_t)KS * 1024 + lane16 + 4096 - 1024 * (c & 3);
+    for (int half = 0; half < 2; ++half) {
+        bool second;
+        const int first = weight_tile(wave * NB + (BOTH ? half * (NB / 2) : 0), second);
+        b_base[half] = reinterpret_cast<const uint8_t*>(second ? p.w2 : p.w) + (size_t)first * KS * 1024 - 4096;
+#pragma unroll
+        for (int c = half * NB / 2; c < (half + 1) * NB / 2 || (NB == 1 && c == 0); ++c)
+            b_off[c] = (uint32_t)(weight_tile(wave * NB + c, second) - first) * (uint32_t)KS * 1024 + lane16 + 4096 - 1024 * (c & 3);
     }
-    // weight scales: a wave requests four tiles' 256 bytes of the round at once, 16 lanes a tile
+    // weight scales: a wave requests four tiles' 256 bytes of the round at once, 16 lanes a tile; waves past the tiles repeat the first ones' request
+    const int wsc_wave = wave & (TILES / 4 - 1);
     const uint8_t* wsc_base;
     {
         bool second;
-        const int tile = weight_tile(wave * 4 + (lane >> 4), second);
+        const int tile = weight_tile(wsc_wave * 4 + (lane >> 4), second);
         wsc_base = reinterpret_cast<const uint8_t*>(second ? p.ws2 : p.ws) + (size_t)tile * KQ * 256 + (lane & 15) * 16;
     }
     const uint8_t* asc_row = p.a_scales + (size_t)(row0 + min(tid & (BM - 1), rows - 1)) * s_pitch;
@@ -148,16 +152,16 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
             if constexpr (WHOLE) tf_mx_dma16<1024 * (OP & 3)>(a_base + (size_t)ks * ROWB, a_off[OP]);
             else tf_mx_dma16<1024 * (OP & 3)>(a_base, a_off[OP] + min((uint32_t)ks * ROWB + a_col[OP], (uint32_t)a_pitch - 16));
         } else {
-            constexpr int C = OP - NA;
+            constexpr int C = OP - NA, H = BOTH && C >= NB / 2 ? 1 : 0;
             if constexpr (C % 4 == 0) tf_mx_m0(lds_stage + A_STAGE + (wave * NB + C) * 1024);
-            if constexpr (WHOLE) tf_mx_dma16<1024 * (C & 3)>(b_base + (size_t)ks * 1024, b_off[C]);
-            else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? b_base + (size_t)ks * 1024 : zeros, ks < KS ? b_off[C] : lane16 + 4096 - 1024 * (C & 3));
+            if constexpr (WHOLE) tf_mx_dma16<1024 * (C & 3)>(b_base[H] + (size_t)ks * 1024, b_off[C]);
+            else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? b_base[H] + (size_t)ks * 1024 : zeros, ks < KS ? b_off[C] : lane16 + 4096 - 1024 * (C & 3));
         }
     };
     const int asc_wave = wave & (BM / 64 - 1);                               // waves past the tile's rows repeat the first ones' request
     auto issue_scales = [&](int kq) {                                        // the MORE requests of a round (kq clamped: the count stays)
         kq = min(kq, KQ - 1);
-        tf_mx_m0(lds_wsc + wave * 1024);
+        tf_mx_m0(lds_wsc + wsc_wave * 1024);
         tf_mx_dma16(wsc_base + (size_t)kq * 256);
         if constexpr (SC == MX_SCALES_32) { tf_mx_m0(lds_asc + asc_wave * 1024); tf_mx_dma16(asc_row + kq * 16); }
         if constexpr (SC == MX_SCALES_128) { tf_mx_m0(lds_asc + asc_wave * 256); tf_mx_dma4(asc_row + kq * 4); }
@@ -171,7 +175,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
         u4v w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = any[4 * j] | (any[4 * j + 1] << 8) | (any[4 * j + 2] << 16) | (any[4 * j + 3] << 24);
-        *reinterpret_cast<u4v*>(s_asc + tid * 4) = w;
+        *reinterpret_cast<u4v*>(s_asc + (tid & (BM - 1)) * 4) = w;               // (threads past the rows repeat the first ones)
     };
 
     // ---- fragments ---------------------------------------------------------------------------------------------------
@@ -244,15 +248,17 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
         tf_static_for<P>([&](auto i_constant) {
             constexpr int I = decltype(i_constant)::value, F = I / FT, T = I % FT;
             tf_mx_mfma<Q, Q>(acc[F][T], wv[X][T], av[X][F], sw[0][T], sa[0][F]);
-            constexpr int R = I * ALL * 4 / (P * 3), R_NEXT = (I + 1) * ALL * 4 / (P * 3);       // within the first three quarters
-            if constexpr (R_NEXT > R && R < ALL) {
-                if constexpr (R < FT) read_w(wv[Y][R], R, next);
-                else if constexpr (R < READS) read_a(av[Y][R - FT], R - FT, next);
-                else if constexpr (R < READS + FT) read_sw(sw[1][R - READS], R - READS);
-                else read_sa(sa[1][R - READS - FT], R - READS - FT);
-            }
-            constexpr int D = I * DATA / P, D_LAST = I == 0 ? -1 : (I - 1) * DATA / P;
-            if constexpr (D != D_LAST) issue(std::integral_constant<int, D>{}, ahead, lds_now);
+            // reads within the first three quarters
+            constexpr int R = I * ALL * 4 / (P * 3) < ALL ? I * ALL * 4 / (P * 3) : ALL, R_NEXT = (I + 1) * ALL * 4 / (P * 3) < ALL ? (I + 1) * ALL * 4 / (P * 3) : ALL;
+            tf_static_for<R_NEXT - R>([&](auto j_constant) {
+                constexpr int J = R + decltype(j_constant)::value;
+                if constexpr (J < FT) read_w(wv[Y][J], J, next);
+                else if constexpr (J < READS) read_a(av[Y][J - FT], J - FT, next);
+                else if constexpr (J < READS + FT) read_sw(sw[1][J - READS], J - READS);
+                else read_sa(sa[1][J - READS - FT], J - READS - FT);
+            });
+            constexpr int D = (I * DATA + P - 1) / P, D_NEXT = ((I + 1) * DATA + P - 1) / P;
+            tf_static_for<D_NEXT - D>([&](auto j_constant) { issue(std::integral_constant<int, D + decltype(j_constant)::value>{}, ahead, lds_now); });
             __builtin_amdgcn_sched_barrier(0);
         });
         stage = next;
@@ -272,37 +278,43 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
 
     // ---- results ---------------------------------------------------------------------------------------------------------
     // Lane (g, r16) of acc[f][t] holds columns 4 g .. 4 g + 3 of tile t for token row 16 f + r16 of the wave.  They pass through LDS as BF16 rows of
-    // 256 bytes (eight-byte chunks permuted by the row: a row's own lanes would all meet in four banks), so that what follows is one short
+    // the wave (gated: the workgroup) (eight-byte chunks permuted by the row: a row's own lanes would all meet in four banks), so that what follows is one short
     // loop over whole 16-byte pieces of rows: written out for every accumulator, its code alone was 50 KiB and ran at the speed of
     // the instruction cache's misses (17 us a tile).
     tf_mx_barrier();                                                         // every wave has read its last stage
     if constexpr (!GATED) {
         constexpr int RB = FT * 32, PIECES = RB / 16;                        // a wave's own rows of 16 FT columns
         uint8_t* own = s_ring + wave * (16 * FM * RB);
-        static_assert(RB == 256 && WAVES * 16 * FM * RB <= NS * STAGE, "rows of 32 chunks");
+        constexpr int MIX = RB / 8 - 2;                                      // the chunk's bits that the row permutes (pairs of chunks stay together)
+        static_assert((RB & (RB - 1)) == 0 && WAVES * 16 * FM * RB <= NS * STAGE, "rows of a power of two of chunks");
 #pragma unroll
         for (int f = 0; f < FM; ++f)
 #pragma unroll
             for (int t = 0; t < FT; ++t)
-                *reinterpret_cast<u2v*>(own + (16 * f + r16) * RB + (((t * 4 + g) ^ (r16 << 1)) << 3)) =
+                *reinterpret_cast<u2v*>(own + (16 * f + r16) * RB + (((t * 4 + g) ^ ((r16 << 1) & MIX)) << 3)) =
                     u2v{tf_pack_bf16(acc[f][t][0], acc[f][t][1]), tf_pack_bf16(acc[f][t][2], acc[f][t][3])};
         const int piece = lane % PIECES, col = tile_n * COLS + wn * FT * 16 + piece * 8;
 #pragma unroll 4
         for (int r = lane / PIECES; r < 16 * FM; r += 64 / PIECES) {
-            const u4v o = *reinterpret_cast<const u4v*>(own + r * RB + (((piece << 1) ^ ((r & 15) << 1)) << 3));
+            const u4v o = *reinterpret_cast<const u4v*>(own + r * RB + (((piece << 1) ^ (((r & 15) << 1) & MIX)) << 3));
             const int row = wm * 16 * FM + r;
             if (row < rows && col < p.n) {
                 uint16_t* to = p.out + (size_t)(row0 + row) * p.out_stride + col;
                 if (p.wide == 2 && col + 8 <= p.n) *reinterpret_cast<u4v*>(to) = o;
-                else {
-                    const int count = min(8, p.n - col);
-                    for (int j = 0; j < count; ++j) to[j] = (uint16_t)(o[j >> 1] >> (16 * (j & 1)));
-                }
+                else
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (p.wide && col + 4 * half + 4 <= p.n) *reinterpret_cast<u2v*>(to + 4 * half) = u2v{o[2 * half], o[2 * half + 1]};
+                        else
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) if (col + 4 * half + j < p.n) to[4 * half + j] = (uint16_t)(o[2 * half + (j >> 1)] >> (16 * (j & 1)));
+                    }
             }
         }
     } else {
         constexpr int HT = FT / 2, RB = COLS * 2, PIECES = RB / 16;          // the workgroup's rows of COLS columns of the activation
-        static_assert(RB == 256 && BM * RB <= NS * STAGE, "rows of 32 chunks");
+        constexpr int MIX = RB / 8 - 2;
+        static_assert((RB & (RB - 1)) == 0 && BM * RB <= NS * STAGE, "rows of a power of two of chunks");
 #pragma unroll
         for (int f = 0; f < FM; ++f) {
             __builtin_amdgcn_sched_barrier(0);
@@ -311,26 +323,38 @@ __global__ void __launch_bounds__(WM * WN * 64, 1) tf_mx_gemm(const MxArgs p, in
                 float v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = tf_mx_swiglu(acc[f][t][i], acc[f][HT + t][i], p.limit);
-                *reinterpret_cast<u2v*>(s_ring + (wm * 16 * FM + 16 * f + r16) * RB + ((((wn * HT + t) * 4 + g) ^ (r16 << 1)) << 3)) =
+                *reinterpret_cast<u2v*>(s_ring + (wm * 16 * FM + 16 * f + r16) * RB + ((((wn * HT + t) * 4 + g) ^ ((r16 << 1) & MIX)) << 3)) =
                     u2v{tf_pack_bf16(v[0], v[1]), tf_pack_bf16(v[2], v[3])};
             }
         }
         tf_mx_barrier();
         const int piece = lane % PIECES, col = tile_n * COLS + piece * 8;
         for (int r = tid / PIECES; r < BM; r += WAVES * 64 / PIECES) {
-            const u4v h = *reinterpret_cast<const u4v*>(s_ring + r * RB + (((piece << 1) ^ ((r & 15) << 1)) << 3));
+            const u4v h = *reinterpret_cast<const u4v*>(s_ring + r * RB + (((piece << 1) ^ (((r & 15) << 1) & MIX)) << 3));
             tf_mx_store_activation(p, h, (size_t)(row0 + r), col, r < rows && col < p.n);
         }
     }
 }
 
+template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
+inline int tf_mx_gemm_tiles(const MxArgs& p, hipStream_t s) {
+    constexpr int ROWS = 16 * FM * WM, COLS = (GATED ? 8 : 16) * FT * WN;
+    const int tiles_m = (p.rows + ROWS - 1) / ROWS, tiles_n = (p.n + COLS - 1) / COLS;
+    const long long total = (long long)tiles_m * tiles_n;
+    if (total > 0x7ffffff0ll) return -1;
+    tf_mx_gemm<FP4A, GATED, SC, FM, FT, WM, WN, NS><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(p, tiles_m, tiles_n);
+    return (int)hipGetLastError();
+}
+#ifndef MX_SIZE
+#define MX_SIZE(p, gated) 2
+#endif
 template <bool FP4A, bool GATED, int SC>
 inline int tf_mx_gemm_go(const MxArgs& p, hipStream_t s) {
-    constexpr int NS = FP4A ? 4 : 3;
-    const int tiles_m = (p.rows + 255) / 256, cols = GATED ? 128 : 256, tiles_n = (p.n + cols - 1) / cols;
-    const long long total = (long long)tiles_m * tiles_n;
-    tf_mx_gemm<FP4A, GATED, SC, 8, 8, 2, 2, NS><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(p, tiles_m, tiles_n);
-    return (int)hipGetLastError();
+    const int size = MX_SIZE(p, GATED);
+    if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, s);
+    if (GATED && p.out_block == 128) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, s);
+    if (size == 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, s);
+    return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, s);
 }
 template <bool FP4A, bool GATED>
 inline int tf_launch_mx_gemm(const MxArgs& p, hipStream_t s) {
