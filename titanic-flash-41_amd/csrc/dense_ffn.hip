@@ -115,7 +115,7 @@ int ca_mxfp4_linear(void* context, int rows, int n, int k, const void* a, const 
     p.a = (const uint8_t*)a; p.a_scales = (const uint8_t*)a_scales; p.w = (const u4v*)w; p.ws = (const uint32_t*)w_scales;
     p.rows = rows; p.n = n; p.k = k; p.block_shift = a_type == CA_MX_E4M3 && c.g.act_block == 128 ? 7 : 5;
     p.out = (uint16_t*)out; p.out_stride = out_stride; p.wide = out_stride % 8 == 0 && aligned(out, 16) ? 2 : out_stride % 4 == 0 && aligned(out, 8) ? 1 : 0;
-    return tf_launch_mx(p, false, a_type == CA_MX_E2M1, (hipStream_t)stream);
+    return tf_launch_mx(p, false, a_type == CA_MX_E2M1, c.cus, (hipStream_t)stream);
 }
 
 int ca_mxfp4_swiglu(void* context, int rows, int inter, int k, const void* a, const void* a_scales, int a_type, const void* up, const void* up_scales,
@@ -136,7 +136,7 @@ int ca_mxfp4_swiglu(void* context, int rows, int inter, int k, const void* a, co
     p.rows = rows; p.n = inter; p.k = k; p.block_shift = a_type == CA_MX_E4M3 && c.g.act_block == 128 ? 7 : 5;
     p.act = (uint16_t*)act; p.codes = (uint8_t*)codes; p.scales = (uint8_t*)scales; p.out_block = block; p.out_fp4 = out_type == CA_MX_E2M1;
     p.limit = c.g.swiglu_limit;
-    return tf_launch_mx(p, true, a_type == CA_MX_E2M1, (hipStream_t)stream);
+    return tf_launch_mx(p, true, a_type == CA_MX_E2M1, c.cus, (hipStream_t)stream);
 }
 
 }  // extern "C"

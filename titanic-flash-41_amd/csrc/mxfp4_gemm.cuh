@@ -26,6 +26,8 @@ __device__ __forceinline__ void tf_mx_dma16(const uint8_t* base, uint32_t offset
 }
 __device__ __forceinline__ void tf_mx_dma16(const uint8_t* from) { asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(from) : "memory"); }
 __device__ __forceinline__ void tf_mx_dma4(const uint8_t* from) { asm volatile("global_load_lds_dword %0, off" ::"v"(from) : "memory"); }
+// One byte a lane, as a word in LDS (only its low byte is used).
+__device__ __forceinline__ void tf_mx_dma1(const uint8_t* from) { asm volatile("global_load_lds_ubyte %0, off" ::"v"(from) : "memory"); }
 template <class F, int... I>
 __device__ __forceinline__ void tf_static_for(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 template <int N, class F>
@@ -63,9 +65,12 @@ __device__ __forceinline__ void tf_mx_settle(v4f (&acc)[FM][FT]) {
 }
 
 // How a row's scales reach the lanes (all end as one register a fragment and round, byte q = k-step q of the round):
-enum { MX_SCALES_32 = 0,      // blocks of 32, k a multiple of 512: 16 bytes a row and round, copied by the memory system
-       MX_SCALES_128 = 1,     // blocks of 128, k a multiple of 512: 4 bytes a row and round, likewise
-       MX_SCALES_ANY = 2 };   // any k: a thread reads its row's bytes one by one a round ahead and writes them to LDS
+enum { MX_SCALES_32 = 0,         // blocks of 32, k a multiple of 512: 16 bytes a row and round, copied by the memory system
+       MX_SCALES_128 = 1,        // blocks of 128, k a multiple of 512: 4 bytes a row and round, likewise
+       MX_SCALES_STEP_32 = 2,    // blocks of 32, k a multiple of 128: 4 bytes a row and k-step
+       MX_SCALES_STEP_128 = 3,   // blocks of 128, any k they divide: 1 byte a row and k-step (a word in LDS)
+       MX_SCALES_ANY = 4 };      // blocks of 32, k no multiple of 128: a thread reads its row's bytes a round ahead and writes them to LDS; its loads are
+                                 // ones the compiler waits for, and with them for every request in flight (two thirds longer a round)
 
 // What the k-steps of the last round past the end of k multiply by: zero codes (a round is four k-steps whatever k is; the loop body then
 // has no branch, which its 256 accumulators would not survive in registers).
@@ -75,7 +80,7 @@ template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
 __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 16 ? 2 : 3) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
     constexpr int WAVES = WM * WN, BM = 16 * FM * WM, TILES = FT * WN, ROWB = FP4A ? 64 : 128;
     constexpr int A_STAGE = BM * ROWB, B_STAGE = TILES * 1024, STAGE = A_STAGE + B_STAGE;
-    constexpr int NA = A_STAGE / 1024 / WAVES, NB = TILES / WAVES, DATA = NA + NB, MORE = SC == MX_SCALES_ANY ? 1 : 2;
+    constexpr int NA = A_STAGE / 1024 / WAVES, NB = TILES / WAVES, DATA = NA + NB, MORE = SC == MX_SCALES_ANY ? 1 : SC >= MX_SCALES_STEP_32 ? 5 : 2;
     constexpr int COLS = (GATED ? TILES / 2 : TILES) * 16, LANES_ROW = ROWB / 16, ROWS_REQ = 64 / LANES_ROW;
     static_assert(NA * WAVES * 1024 == A_STAGE && NB * WAVES == TILES && TILES % 4 == 0 && TILES <= 4 * WAVES && BM % 64 == 0 && BM <= WAVES * 64, "whole requests a wave");
     typedef typename MxFragment<FP4A>::type Fragment;
@@ -101,7 +106,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     const uint32_t lds_ring = tf_mx_lds(s_ring), lds_wsc = tf_mx_lds(s_wsc), lds_asc = tf_mx_lds(s_asc);
     // Every request is a scalar base that moves on with the k-step plus the lane's own offset; four requests share an m0, so a request's
     // offset holds 1,024 bytes for every one before it in its four less (and the bases point 4,096 bytes before their data).
-    constexpr bool WHOLE = SC != MX_SCALES_ANY;                              // k is whole rounds: no request needs a bound
+    constexpr bool ROUNDS = SC <= MX_SCALES_128, STEPS = SC != MX_SCALES_ANY;   // k is whole rounds / k-steps: no request / no lane needs a bound
     const uint8_t* a_base = p.a + (size_t)row0 * a_pitch - 4096;
     uint32_t a_off[NA], a_col[NA];
 #pragma unroll
@@ -110,7 +115,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         const int swz = FP4A ? ((r >> 1) & 3) ^ (r >> 3) : (r & 7) ^ (r >> 3);
         a_col[c] = (uint32_t)((lane % LANES_ROW) ^ swz) * 16;
         // past the last row: that row again, never stored
-        a_off[c] = (uint32_t)min(row, rows - 1) * (uint32_t)a_pitch + 4096 - 1024 * (c & 3) + (WHOLE ? a_col[c] : 0);
+        a_off[c] = (uint32_t)min(row, rows - 1) * (uint32_t)a_pitch + 4096 - 1024 * (c & 3) + (STEPS ? a_col[c] : 0);
     }
     // weight tile T of the workgroup (gated: a wave's FT tiles are FT / 2 of `up`, then the same columns' of `gate`)
     auto weight_tile = [&](int T, bool& second) {
@@ -149,12 +154,12 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         constexpr int OP = decltype(op_constant)::value;
         if constexpr (OP < NA) {
             if constexpr (OP % 4 == 0) tf_mx_m0(lds_stage + (wave * NA + OP) * 1024);
-            if constexpr (WHOLE) tf_mx_dma16<1024 * (OP & 3)>(a_base + (size_t)ks * ROWB, a_off[OP]);
+            if constexpr (STEPS) tf_mx_dma16<1024 * (OP & 3)>(a_base + (size_t)(ROUNDS ? ks : min(ks, KS - 1)) * ROWB, a_off[OP]);
             else tf_mx_dma16<1024 * (OP & 3)>(a_base, a_off[OP] + min((uint32_t)ks * ROWB + a_col[OP], (uint32_t)a_pitch - 16));
         } else {
             constexpr int C = OP - NA, H = BOTH && C >= NB / 2 ? 1 : 0;
             if constexpr (C % 4 == 0) tf_mx_m0(lds_stage + A_STAGE + (wave * NB + C) * 1024);
-            if constexpr (WHOLE) tf_mx_dma16<1024 * (C & 3)>(b_base[H] + (size_t)ks * 1024, b_off[C]);
+            if constexpr (ROUNDS) tf_mx_dma16<1024 * (C & 3)>(b_base[H] + (size_t)ks * 1024, b_off[C]);
             else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? b_base[H] + (size_t)ks * 1024 : zeros, ks < KS ? b_off[C] : lane16 + 4096 - 1024 * (C & 3));
         }
     };
@@ -165,6 +170,15 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         tf_mx_dma16(wsc_base + (size_t)kq * 256);
         if constexpr (SC == MX_SCALES_32) { tf_mx_m0(lds_asc + asc_wave * 1024); tf_mx_dma16(asc_row + kq * 16); }
         if constexpr (SC == MX_SCALES_128) { tf_mx_m0(lds_asc + asc_wave * 256); tf_mx_dma4(asc_row + kq * 4); }
+        if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) {     // [k-step][row]
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int ks = min(4 * kq + q, KS - 1);
+                tf_mx_m0(lds_asc + q * (BM * 4) + asc_wave * 256);
+                if constexpr (SC == MX_SCALES_STEP_32) tf_mx_dma4(asc_row + ks * 4);
+                else tf_mx_dma1(asc_row + ks);
+            }
+        }
     };
     uint32_t any[16];
     auto read_scales = [&](int kq) {                                         // MX_SCALES_ANY: this thread's row, one byte a block of 32
@@ -202,8 +216,10 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         const int row = wm * 16 * FM + 16 * f + r16;
         if constexpr (SC == MX_SCALES_128) to = s_asc[row];
         else {                                                                // byte g of each k-step's word
-            const u4v w = *reinterpret_cast<const u4v*>(s_asc + row * 4);
-            const uint32_t pick = (uint32_t)g | ((uint32_t)(4 + g) << 8);     // bytes g of the second and the first operand
+            u4v w;
+            if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) w = u4v{s_asc[row], s_asc[BM + row], s_asc[2 * BM + row], s_asc[3 * BM + row]};
+            else w = *reinterpret_cast<const u4v*>(s_asc + row * 4);
+            const uint32_t byte = SC == MX_SCALES_STEP_128 ? 0 : (uint32_t)g, pick = byte | ((4 + byte) << 8);       // of the second and the first operand
             const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], pick), hi = __builtin_amdgcn_perm(w[3], w[2], pick);
             to = (lo & 0xffffu) | (hi << 16);
         }
@@ -345,27 +361,49 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, hipStream_t s) {
     tf_mx_gemm<FP4A, GATED, SC, FM, FT, WM, WN, NS><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(p, tiles_m, tiles_n);
     return (int)hipGetLastError();
 }
-#ifndef MX_SIZE
-#define MX_SIZE(p, gated) 2
+// The tile's size.  A 256 x 256 tile takes 54 us of a CU at k = 4,096 (E4M3 rows), one of 128 x 128 (two a CU at once) 14.5 us, one of 64 x 64
+// 6 us (plus 3 us once): the large ones read LDS and L2 least for a product, the small ones give every CU something to do.
+//  - 64 x 64 while they are at most two a CU: 256 rows x 4,096: 8.5 us, against 14.8 (128) and 40 (256); 512 rows: 13.6, 15.8, 41
+//  - 256 x 256 where whole rounds of them cost less than whole rounds of 128 x 128, a quarter of the work at 15 / 16 of the time: 4,096 rows x
+//    4,096: 54 us against 58; but 2,048 rows (half the CUs without a tile) 46 against 30, 16 x 18 tiles (two rounds for 1.1) 74 against 70
+//  - else 128 x 128: 1,024 rows: 18.8 us, against 25.5 (64) and 42 (256)
+// Blocks of 128 columns of a gated product's codes need the tile's columns to be whole blocks: 64 rows x 128 columns in place of the two
+// smaller ones.
+inline int tf_mx_tile_size(const MxArgs& p, bool gated, int cus) {
+#ifdef MX_SIZE
+    return MX_SIZE;
 #endif
+    auto tiles = [&](int rows, int cols) { return (long long)((p.rows + rows - 1) / rows) * ((p.n * (gated ? 2ll : 1ll) + cols - 1) / cols); };
+    auto rounds = [&](long long t) { return (t + cus - 1) / cus; };
+    if (tiles(64, 64) <= 2 * cus) return 0;
+    return 15 * rounds(tiles(256, 256)) <= 4 * rounds(tiles(128, 128)) ? 2 : 1;
+}
 template <bool FP4A, bool GATED, int SC>
-inline int tf_mx_gemm_go(const MxArgs& p, hipStream_t s) {
-    const int size = MX_SIZE(p, GATED);
+inline int tf_mx_gemm_go(const MxArgs& p, int cus, hipStream_t s) {
+    const int size = tf_mx_tile_size(p, GATED, cus);
     if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, s);
-    if (GATED && p.out_block == 128) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, s);
+    if constexpr (GATED)
+        if (p.out_block == 128) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, s);
     if (size == 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, s);
     return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, s);
 }
 template <bool FP4A, bool GATED>
-inline int tf_launch_mx_gemm(const MxArgs& p, hipStream_t s) {
-    if (p.k % 512 == 0 && p.block_shift == 5 && (size_t)p.a_scales % 16 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_32>(p, s);
-    if constexpr (!FP4A)
-        if (p.k % 512 == 0 && p.block_shift == 7 && (size_t)p.a_scales % 4 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_128>(p, s);
-    return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_ANY>(p, s);
+inline int tf_launch_mx_gemm(const MxArgs& p, int cus, hipStream_t s) {
+    const size_t at = (size_t)p.a_scales;
+    if (p.block_shift == 5) {
+        if (p.k % 512 == 0 && at % 16 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_32>(p, cus, s);
+        if (p.k % 128 == 0 && at % 4 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_STEP_32>(p, cus, s);
+        return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_ANY>(p, cus, s);
+    }
+    if constexpr (!FP4A) {
+        if (p.k % 512 == 0 && at % 4 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_128>(p, cus, s);
+        return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_STEP_128>(p, cus, s);
+    }
+    return -1;
 }
 // Both regimes of the products.
-inline int tf_launch_mx(const MxArgs& p, bool gated, bool fp4_rows, hipStream_t s) {
+inline int tf_launch_mx(const MxArgs& p, bool gated, bool fp4_rows, int cus, hipStream_t s) {
     if (p.rows <= 64) return fp4_rows ? tf_launch_mx_stream<true>(p, gated, s) : tf_launch_mx_stream<false>(p, gated, s);
-    if (gated) return fp4_rows ? tf_launch_mx_gemm<true, true>(p, s) : tf_launch_mx_gemm<false, true>(p, s);
-    return fp4_rows ? tf_launch_mx_gemm<true, false>(p, s) : tf_launch_mx_gemm<false, false>(p, s);
+    if (gated) return fp4_rows ? tf_launch_mx_gemm<true, true>(p, cus, s) : tf_launch_mx_gemm<false, true>(p, cus, s);
+    return fp4_rows ? tf_launch_mx_gemm<true, false>(p, cus, s) : tf_launch_mx_gemm<false, false>(p, cus, s);
 }
