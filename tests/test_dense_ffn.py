@@ -486,6 +486,32 @@ def test_linear(gpu, kind, block, rows, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,block", [(0, 32), (0, 128), (1, 32)])
+@pytest.mark.parametrize("rows,n,k", [(1090, 2100, 416), (1090, 2100, 640), (1025, 2304, 512), (4090, 4090, 512), (4090, 4090, 640), (4090, 4084, 544)])
+def test_linear_large_tiles(gpu, kind, block, rows, n, k):
+    """Enough tiles that the larger ones are chosen, ragged in both directions.  The reference runs on the device in float64."""
+    g = gpu(block)
+    if block == 128:
+        k = -(-k // 128) * 128
+    a, a_scales, av = activations(g, kind, rows, k)
+    words, scales = mxfp4("w", n, k)
+    wv = values4(words, scales)
+    out = g.linear(rows, n, k, a, a_scales, kind, g.prepare(words, scales)).double()
+    want, bound = device_product(av, wv, kind)
+    assert bool(((out - want).abs() <= want.abs() * 2.0 ** -8 + bound).all())
+
+
+def device_product(av, wv, kind):
+    """The product and product_error() on the device, in float64."""
+    a, w = torch.from_numpy(av).cuda(), torch.from_numpy(wv).cuda()
+    e = (a.abs() @ w.abs().t().contiguous()) * 2.0 ** -19
+    if kind == native.MX_E4M3:
+        most = lambda v: v.abs().reshape(v.shape[0], -1, 8).amax(dim=2)
+        e += (most(a) @ most(w).t().contiguous()) * (7 * 2.0 ** -13)
+    return a @ w.t().contiguous(), e
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [0, 1])
 def test_linear_exact_small_whole_numbers(gpu, kind):
     """Whole-number operands whose sums every format holds: no rounding anywhere, so every index of the product is checked exactly."""
@@ -589,6 +615,33 @@ def test_swiglu(gpu, kind, block, rows, inter, k):
     h4, w4, s4 = g.swiglu(rows, inter, k, a, a_scales, kind, up, gate, out_kind=native.MX_E2M1)
     words, scales = g.quant(h4)
     assert torch.equal(h4, h) and torch.equal(w4, words) and torch.equal(s4, scales)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,block", [(0, 32), (0, 128), (1, 32), (1, 128)])
+@pytest.mark.parametrize("rows,inter,k", [(1090, 1152, 640), (4090, 2016, 512), (4090, 2016, 416)])
+def test_swiglu_large_tiles(gpu, kind, block, rows, inter, k):
+    g = gpu(block)
+    if block == 128:
+        inter, k = -(-inter // 128) * 128, -(-k // 128) * 128
+    a, a_scales, av = activations(g, kind, rows, k, std=2.0)
+    ups, gates = mxfp4("up", inter, k, std=0.1), mxfp4("gate", inter, k, std=0.1)
+    up, gate = g.prepare(*ups), g.prepare(*gates)
+    h, c, s = g.swiglu(rows, inter, k, a, a_scales, kind, up, gate)
+    (gv, eg), (uv, eu) = device_product(av, values4(*gates), kind), device_product(av, values4(*ups), kind)
+    gc, uc = gv.clamp(max=LIMIT), uv.clamp(-LIMIT, LIMIT)
+    silu = gc / (1.0 + torch.exp(-gc))
+    want = silu * uc
+    moved = 1.1 * eg * (uc.abs() + eu) + silu.abs() * eu + want.abs() * (gc.abs() + 4) * 2.0 ** -23        # as swiglu_want()
+    assert bool(((h.double() - want).abs() <= want.abs() * 2.0 ** -8 + moved).all())
+    codes, bytes_ = quant8(f64(h), block)
+    assert np.array_equal(s.cpu().numpy(), bytes_)
+    assert np.array_equal(c.cpu().view(torch.float8_e4m3fn).to(torch.float64).numpy(), codes)
+    h2, w4, s4 = g.swiglu(rows, inter, k, a, a_scales, kind, up, gate, out_kind=native.MX_E2M1)
+    words, scales = g.quant(h2)
+    assert torch.equal(h2, h) and torch.equal(w4, words) and torch.equal(s4, scales)
+    _, c3, s3 = g.swiglu(rows, inter, k, a, a_scales, kind, up, gate, act=False)
+    assert torch.equal(c3, c) and torch.equal(s3, s)
 
 
 @pytest.mark.gpu

@@ -1,6 +1,6 @@
-// Products with prepared MXFP4 weights for many rows: tiles of 256 rows x 256 weight rows on the matrix cores.
+// Products with prepared MXFP4 weights for many rows: tiles of 256 (128, 64) rows x as many weight rows on the matrix cores.
 //
-// A workgroup of WM x WN waves (one a SIMD); a wave holds 16 FM token rows x 16 FT weight rows in 4 FM FT accumulator registers a lane.
+// A workgroup of WM x WN = 4 waves (one a SIMD); a wave holds 16 FM token rows x 16 FT weight rows in 4 FM FT accumulator registers a lane.
 // A k-step is 128 columns: FM FT instructions of 16 x 16 x 128 a wave.  Both operands come into LDS by global_load_lds in a ring of NS
 // stages, requested NS k-steps ahead.  In k-step s the wave multiplies from registers (one set), reads k-step s + 1 from LDS into
 // the other set between its products, and requests k-step s + NS into the stage that k-step s lay in; one barrier a k-step, at its
@@ -69,8 +69,7 @@ enum { MX_SCALES_32 = 0,         // blocks of 32, k a multiple of 512: 16 bytes 
        MX_SCALES_128 = 1,        // blocks of 128, k a multiple of 512: 4 bytes a row and round, likewise
        MX_SCALES_STEP_32 = 2,    // blocks of 32, k a multiple of 128: 4 bytes a row and k-step
        MX_SCALES_STEP_128 = 3,   // blocks of 128, any k they divide: 1 byte a row and k-step (a word in LDS)
-       MX_SCALES_ANY = 4 };      // blocks of 32, k no multiple of 128: a thread reads its row's bytes a round ahead and writes them to LDS; its loads are
-                                 // ones the compiler waits for, and with them for every request in flight (two thirds longer a round)
+       MX_SCALES_ANY = 4 };      // blocks of 32, k no multiple of 128: 1 byte a row and block, likewise (16 words a row: no room beside 256 x 256 tiles)
 
 // What the k-steps of the last round past the end of k multiply by: zero codes (a round is four k-steps whatever k is; the loop body then
 // has no branch, which its 256 accumulators would not survive in registers).
@@ -80,13 +79,13 @@ template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
 __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 16 ? 2 : 3) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
     constexpr int WAVES = WM * WN, BM = 16 * FM * WM, TILES = FT * WN, ROWB = FP4A ? 64 : 128;
     constexpr int A_STAGE = BM * ROWB, B_STAGE = TILES * 1024, STAGE = A_STAGE + B_STAGE;
-    constexpr int NA = A_STAGE / 1024 / WAVES, NB = TILES / WAVES, DATA = NA + NB, MORE = SC == MX_SCALES_ANY ? 1 : SC >= MX_SCALES_STEP_32 ? 5 : 2;
+    constexpr int NA = A_STAGE / 1024 / WAVES, NB = TILES / WAVES, DATA = NA + NB, MORE = SC == MX_SCALES_ANY ? 1 + BM / 4 / WAVES : SC >= MX_SCALES_STEP_32 ? 5 : 2;
     constexpr int COLS = (GATED ? TILES / 2 : TILES) * 16, LANES_ROW = ROWB / 16, ROWS_REQ = 64 / LANES_ROW;
     static_assert(NA * WAVES * 1024 == A_STAGE && NB * WAVES == TILES && TILES % 4 == 0 && TILES <= 4 * WAVES && BM % 64 == 0 && BM <= WAVES * 64, "whole requests a wave");
     typedef typename MxFragment<FP4A>::type Fragment;
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NS * STAGE];
     __shared__ __attribute__((aligned(1024))) uint32_t s_wsc[TILES * 64];
-    __shared__ __attribute__((aligned(1024))) uint32_t s_asc[SC == MX_SCALES_128 ? BM : BM * 4];
+    __shared__ __attribute__((aligned(1024))) uint32_t s_asc[SC == MX_SCALES_128 ? BM : SC == MX_SCALES_ANY ? BM * 16 : BM * 4];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, g = lane >> 4, r16 = lane & 15;
@@ -179,17 +178,14 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
                 else tf_mx_dma1(asc_row + ks);
             }
         }
-    };
-    uint32_t any[16];
-    auto read_scales = [&](int kq) {                                         // MX_SCALES_ANY: this thread's row, one byte a block of 32
+        if constexpr (SC == MX_SCALES_ANY) {                                 // [block of the round][row]; request i of the wave's: block i / (BM / 64), 64 rows
 #pragma unroll
-        for (int j = 0; j < 16; ++j) any[j] = asc_row[min((kq * 512 + j * 32) >> p.block_shift, s_pitch - 1)];
-    };
-    auto write_scales = [&]() {
-        u4v w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = any[4 * j] | (any[4 * j + 1] << 8) | (any[4 * j + 2] << 16) | (any[4 * j + 3] << 24);
-        *reinterpret_cast<u4v*>(s_asc + (tid & (BM - 1)) * 4) = w;               // (threads past the rows repeat the first ones)
+            for (int i = 0; i < MORE - 1; ++i) {
+                const int request = wave * (MORE - 1) + i, block = request / (BM / 64), row = request % (BM / 64) * 64;
+                tf_mx_m0(lds_asc + (block * BM + row) * 4);
+                tf_mx_dma1(p.a_scales + (size_t)(row0 + min(row + lane, rows - 1)) * s_pitch + min(16 * kq + block, s_pitch - 1));
+            }
+        }
     };
 
     // ---- fragments ---------------------------------------------------------------------------------------------------
@@ -217,9 +213,10 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         if constexpr (SC == MX_SCALES_128) to = s_asc[row];
         else {                                                                // byte g of each k-step's word
             u4v w;
-            if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) w = u4v{s_asc[row], s_asc[BM + row], s_asc[2 * BM + row], s_asc[3 * BM + row]};
+            if constexpr (SC == MX_SCALES_ANY) w = u4v{s_asc[g * BM + row], s_asc[(4 + g) * BM + row], s_asc[(8 + g) * BM + row], s_asc[(12 + g) * BM + row]};
+            else if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) w = u4v{s_asc[row], s_asc[BM + row], s_asc[2 * BM + row], s_asc[3 * BM + row]};
             else w = *reinterpret_cast<const u4v*>(s_asc + row * 4);
-            const uint32_t byte = SC == MX_SCALES_STEP_128 ? 0 : (uint32_t)g, pick = byte | ((4 + byte) << 8);       // of the second and the first operand
+            const uint32_t byte = SC >= MX_SCALES_STEP_128 ? 0 : (uint32_t)g, pick = byte | ((4 + byte) << 8);       // of the second and the first operand
             const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], pick), hi = __builtin_amdgcn_perm(w[3], w[2], pick);
             to = (lo & 0xffffu) | (hi << 16);
         }
@@ -227,7 +224,6 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     auto read_sw = [&](uint32_t& to, int t) { to = s_wsc[(wn * FT + t) * 64 + lane]; };
 
     // ---- the first k-steps ---------------------------------------------------------------------------------------------
-    if constexpr (SC == MX_SCALES_ANY) { read_scales(0); write_scales(); }
     issue_scales(0);
 #pragma unroll
     for (int d = 0; d < NS; ++d) tf_static_for<DATA>([&](auto op) { issue(op, d, lds_ring + d * STAGE); });
@@ -250,11 +246,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         const int next = NS == 4 ? (Q + 1) & 3 : (stage + 1 == NS ? 0 : stage + 1), now = NS == 4 ? Q : stage;
         tf_mx_wait<behind(Q)>();
         tf_mx_barrier();
-        if constexpr (Q == 0) {
-            issue_scales((ks >> 2) + 1);
-            if constexpr (SC == MX_SCALES_ANY) read_scales(min((ks >> 2) + 1, KQ - 1));
-        }
-        if constexpr (Q == 2 && SC == MX_SCALES_ANY) write_scales();
+        if constexpr (Q == 0) issue_scales((ks >> 2) + 1);
         const int ahead = min(ks + NS, 4 * KQ - 1);                          // behind the last: that one again, never read
         const uint32_t lds_now = lds_ring + now * STAGE;
         // Product i (fragment i / FT, tile i % FT); behind it, spread over the step, what the next k-step needs from LDS (weights first) and the
@@ -368,11 +360,9 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, hipStream_t s) {
 //    4,096: 54 us against 58; but 2,048 rows (half the CUs without a tile) 46 against 30, 16 x 18 tiles (two rounds for 1.1) 74 against 70
 //  - else 128 x 128: 1,024 rows: 18.8 us, against 25.5 (64) and 42 (256)
 // Blocks of 128 columns of a gated product's codes need the tile's columns to be whole blocks: 64 rows x 128 columns in place of the two
-// smaller ones.
+// smaller ones, or, where 64 x 64 would be chosen and the activation goes to memory too, its codes in a launch of their own behind those
+// (64 rows x 2,048 x 4,096: 15.2 -> 9.6 us).
 inline int tf_mx_tile_size(const MxArgs& p, bool gated, int cus) {
-#ifdef MX_SIZE
-    return MX_SIZE;
-#endif
     auto tiles = [&](int rows, int cols) { return (long long)((p.rows + rows - 1) / rows) * ((p.n * (gated ? 2ll : 1ll) + cols - 1) / cols); };
     auto rounds = [&](long long t) { return (t + cus - 1) / cus; };
     if (tiles(64, 64) <= 2 * cus) return 0;
@@ -381,10 +371,19 @@ inline int tf_mx_tile_size(const MxArgs& p, bool gated, int cus) {
 template <bool FP4A, bool GATED, int SC>
 inline int tf_mx_gemm_go(const MxArgs& p, int cus, hipStream_t s) {
     const int size = tf_mx_tile_size(p, GATED, cus);
-    if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, s);
+    if constexpr (SC != MX_SCALES_ANY)
+        if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, s);
     if constexpr (GATED)
-        if (p.out_block == 128) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, s);
-    if (size == 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, s);
+        if (p.codes != nullptr && p.out_block == 128) {
+            if (size == 0 && p.act != nullptr) {
+                MxArgs first = p;
+                first.codes = first.scales = nullptr;
+                const int status = tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(first, s);
+                return status ? status : tf_launch_mx_codes(p, s);
+            }
+            return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, s);
+        }
+    if (size >= 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, s);
     return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, s);
 }
 template <bool FP4A, bool GATED>
@@ -401,9 +400,11 @@ inline int tf_launch_mx_gemm(const MxArgs& p, int cus, hipStream_t s) {
     }
     return -1;
 }
-// Both regimes of the products.
+// Both regimes of the products.  The streaming kernel reads every weight once for all its rows, but each workgroup reads all the rows: it takes
+// up to 32 (4,096 x 4,096: 24 rows 5.2 us against 6.9 of the 64 x 64 tiles, 40 rows 7.9 against 6.9), and 16 of a gated product, which has twice
+// the weights a column (2,048 x 4,096: 16 rows 6.2 us against 7.6, 24 rows 8.3 against 7.6).
 inline int tf_launch_mx(const MxArgs& p, bool gated, bool fp4_rows, int cus, hipStream_t s) {
-    if (p.rows <= 64) return fp4_rows ? tf_launch_mx_stream<true>(p, gated, s) : tf_launch_mx_stream<false>(p, gated, s);
+    if (p.rows <= (gated ? 16 : 32)) return fp4_rows ? tf_launch_mx_stream<true>(p, gated, cus, s) : tf_launch_mx_stream<false>(p, gated, cus, s);
     if (gated) return fp4_rows ? tf_launch_mx_gemm<true, true>(p, cus, s) : tf_launch_mx_gemm<false, true>(p, cus, s);
     return fp4_rows ? tf_launch_mx_gemm<true, false>(p, cus, s) : tf_launch_mx_gemm<false, false>(p, cus, s);
 }

@@ -6,6 +6,7 @@
 // are decoded and both scales applied in the matrix core, sums are FP32.
 #pragma once
 #include "mxfp4_codec.cuh"
+#include <type_traits>
 
 struct MxArgs {
     const uint8_t *a, *a_scales;
@@ -24,20 +25,6 @@ struct MxArgs {
     float limit;
 };
 
-// The byte of lane group g at k-step ks of a row's 16-byte pieces.  Columns past k (the last step of a k that is no multiple of
-// 128) meet zero weights; the lane then reads its row's last piece again, so that nothing outside the row is touched and a
-// NaN can enter the sum only from the row itself, whose result it is anyway.
-template <bool FP4A>
-__device__ __forceinline__ v8i tf_mx_row_fragment(const uint8_t* row, int ks, int g, int k) {
-    if constexpr (FP4A) {
-        const u4v a = *reinterpret_cast<const u4v*>(row + min(ks * 64 + g * 16, (k >> 1) - 16));
-        return v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-    } else {
-        const u4v a = *reinterpret_cast<const u4v*>(row + min(ks * 128 + g * 16, k - 16));
-        const u4v b = *reinterpret_cast<const u4v*>(row + min(ks * 128 + 64 + g * 16, k - 16));
-        return v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-    }
-}
 template <bool FP4A, int Q>
 __device__ __forceinline__ v4f tf_mx_product(const u4v& w, const v8i& a, const v4f& c, uint32_t scale_w, uint32_t scale_a) {
     const v8i wv = v8i{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
@@ -74,18 +61,27 @@ __device__ __forceinline__ void tf_mx_store_activation(const MxArgs& p, const u4
     }
 }
 
+// Units a batch: what 128 (16 waves) or 256 (8 waves) registers a lane and 160 KiB of LDS hold.
+constexpr int tf_mx_units(bool gated) { return gated ? 1 : 2; }
 // A workgroup: NW column groups of CT 16-column tiles (gated: of both matrices) x MT 16-row tiles; its waves share out the column
-// groups and, within one, the rounds of four k-steps (wave kw takes rounds kw, kw + KW, ..).  Partial sums meet in LDS and are
-// added in the order of the waves.
-template <bool FP4A, bool GATED, int CT, int MT, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 512 : 1024) tf_mx_stream(const MxArgs p) {
-    constexpr int T = GATED ? 2 * CT : CT, COLS = NW * CT * 16;
+// groups and, within one, the units of two k-steps (wave kw takes units kw, kw + KW, ..), UNITS of them at a time, all of whose loads are
+// in flight before the first product.  Partial sums meet in LDS and are added in the order of the waves.
+//
+// Token rows pass through LDS (a region a wave, so no barrier): the lanes that load a row's 128 bytes of a k-step are neighbours, eight rows
+// (E2M1: sixteen) an instruction.  Loaded straight in the matrix instruction's order, sixteen neighbouring lanes want sixteen different
+// rows, each 16-byte piece is a cache look-up of its own, and 16 rows of 4,096 columns cost a launch 3 us.  A row's scales come as one word a
+// k-step, lane group g holding that of the batch's k-step g.
+template <bool FP4A, bool GATED, int CT, int MT, int NW, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) tf_mx_stream(const MxArgs p) {
+    constexpr int T = GATED ? 2 * CT : CT, COLS = NW * CT * 16, UNITS = tf_mx_units(GATED);
+    constexpr int ROWB = FP4A ? 64 : 128, LOADS = ROWB / 64, LANES_ROW = ROWB / 16, OWN = UNITS * 2 * MT * 16 * ROWB;
     extern __shared__ __attribute__((aligned(16))) uint8_t s_dynamic[];
-    v4f* s_part = reinterpret_cast<v4f*>(s_dynamic);                            // [wave][T][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int nw = wave % NW, kw = wave / NW, KW = waves / NW, g = lane >> 4, r16 = lane & 15;
+    uint8_t* s_a = s_dynamic + wave * OWN;                                       // [unit][k-step][MT][16 rows][ROWB], the wave's own
+    v4f* s_part = reinterpret_cast<v4f*>(s_dynamic);                             // [wave][T][64]: behind the last product
     float* s_h = reinterpret_cast<float*>(s_part + waves * T * 64);              // gated: [16][COLS + 4]
-    const int KS = (p.k + 127) >> 7, KQ = (p.k + 511) >> 9, tiles = (p.n + 15) >> 4;
+    const int KS = (p.k + 127) >> 7, KQ = (p.k + 511) >> 9, KU = (KS + 1) >> 1, tiles = (p.n + 15) >> 4;
     const int tile0 = (blockIdx.x * NW + nw) * CT, row0 = blockIdx.y * (16 * MT);
     const int a_pitch = FP4A ? p.k >> 1 : p.k, s_pitch = p.k >> p.block_shift;
 
@@ -98,42 +94,113 @@ __global__ void __launch_bounds__(NW == 1 ? 512 : 1024) tf_mx_stream(const MxArg
         w[t] = (second ? p.w2 : p.w) + tile * KS * 64 + lane;
         ws[t] = (second ? p.ws2 : p.ws) + tile * KQ * 64 + lane;
     }
-    const uint8_t *a[MT], *as[MT];
+    // loads of token rows: lane l takes 16 bytes (l % LANES_ROW) of row l / LANES_ROW; in LDS a row's pieces are permuted by the row (banks)
+    auto swizzle = [](int r) { return FP4A ? ((r >> 1) & 3) ^ (r >> 3) : (r & 7) ^ (r >> 3); };
+    const uint8_t *a[MT][LOADS], *as[MT];
+    const uint32_t a_col = (uint32_t)(lane % LANES_ROW) * 16;
+    uint32_t to_lds[LOADS];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const size_t row = min(row0 + 16 * m + r16, p.rows - 1);                  // past the last row: that row again, never stored
-        a[m] = p.a + row * a_pitch;
-        as[m] = p.a_scales + row * s_pitch;
+    for (int c = 0; c < LOADS; ++c) {
+        const int r = c * (64 / LANES_ROW) + lane / LANES_ROW;
+        to_lds[c] = (uint32_t)(r * ROWB + (((lane % LANES_ROW) ^ swizzle(r)) << 4));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) a[m][c] = p.a + (size_t)min(row0 + 16 * m + r, p.rows - 1) * a_pitch;   // past the last row: that row again, never stored
     }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) as[m] = p.a_scales + (size_t)min(row0 + 16 * m + r16, p.rows - 1) * s_pitch;
+    const uint32_t from_lds = (uint32_t)(r16 * ROWB + ((g ^ swizzle(r16)) << 4));
+    const bool words = p.block_shift == 5 && p.k % 128 == 0 && ((size_t)p.a_scales & 3) == 0;
     v4f acc[MT][T];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[m][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int kq = kw; kq < KQ; kq += KW) {
-        uint32_t sw[T];
+    // U units from unit u on, KW apart, of two k-steps each (the last one of an odd k alone: `odd`)
+    auto units = [&](auto count, auto steps, int u) {
+        constexpr int U = decltype(count)::value, S = decltype(steps)::value;
+        u4v wv[U][S][T], ar[U][S][MT][LOADS];
+        uint32_t sw[U][T], sr[MT];
 #pragma unroll
-        for (int t = 0; t < T; ++t) sw[t] = ws[t][kq * 64];
-        auto step = [&](auto q_constant) {
-            constexpr int Q = decltype(q_constant)::value;
-            const int ks = 4 * kq + Q;
-            if (ks >= KS) return;
-            u4v wv[T];
+        for (int i = 0; i < U; ++i) {
+            const int unit = u + i * KW;
 #pragma unroll
-            for (int t = 0; t < T; ++t) wv[t] = w[t][ks * 64];
+            for (int t = 0; t < T; ++t) sw[i][t] = ws[t][(unit >> 1) * 64];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const v8i av = tf_mx_row_fragment<FP4A>(a[m], ks, g, p.k);
-                const uint32_t sa = as[m][min((ks * 128 + g * 32) >> p.block_shift, s_pitch - 1)];
+            for (int q = 0; q < S; ++q) {
+                const int ks = 2 * unit + q;
 #pragma unroll
-                for (int t = 0; t < T; ++t) acc[m][t] = tf_mx_product<FP4A, Q>(wv[t], av, acc[m][t], sw[t], sa);
+                for (int t = 0; t < T; ++t) wv[i][q][t] = w[t][ks * 64];
+                // Columns past k (the last step of a k that is no multiple of 128) meet zero weights; the lane then reads its row's last piece
+                // again, so that nothing outside the row is touched and a NaN can enter the sum only from the row itself.
+                const uint32_t at = min((uint32_t)ks * ROWB + a_col, (uint32_t)a_pitch - 16);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int c = 0; c < LOADS; ++c) ar[i][q][m][c] = *reinterpret_cast<const u4v*>(a[m][c] + at);
+            }
+        }
+        const int mine = min(2 * (u + (U == 2 ? (g >> 1) * KW : 0)) + (g & 1), KS - 1);      // the k-step whose scales this lane group loads
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (words) sr[m] = *reinterpret_cast<const uint32_t*>(as[m] + mine * 4);
+            else {
+                sr[m] = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sr[m] |= (uint32_t)as[m][min((mine * 128 + j * 32) >> p.block_shift, s_pitch - 1)] << (8 * j);
+            }
+        }
+        asm volatile("" ::: "memory");               // the previous batch's reads of the wave's LDS region come before these writes, theirs after them
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int q = 0; q < S; ++q)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int c = 0; c < LOADS; ++c) *reinterpret_cast<u4v*>(s_a + ((i * 2 + q) * MT + m) * (16 * ROWB) + to_lds[c]) = ar[i][q][m][c];
+        asm volatile("" ::: "memory");
+        auto fragment = [&](int i, int q, int m) {
+            const uint8_t* at = s_a + ((i * 2 + q) * MT + m) * (16 * ROWB);
+            const u4v lo = *reinterpret_cast<const u4v*>(at + from_lds);
+            if constexpr (FP4A) return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
+            else {
+                const u4v hi = *reinterpret_cast<const u4v*>(at + (from_lds ^ 64));
+                return v8i{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
             }
         };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
-    }
+        auto scale = [&](int i, int q, int m) { return (uint32_t)__shfl((int)sr[m], (i * 2 + q) * 16 + r16) >> (8 * g); };
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int shift = ((u + i * KW) & 1) * 16;                           // the unit's two bytes of its round's four
+            uint32_t sh[T];
+#pragma unroll
+            for (int t = 0; t < T; ++t) sh[t] = sw[i][t] >> shift;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const v8i av = fragment(i, 0, m);
+                const uint32_t sa = scale(i, 0, m);
+#pragma unroll
+                for (int t = 0; t < T; ++t) acc[m][t] = tf_mx_product<FP4A, 0>(wv[i][0][t], av, acc[m][t], sh[t], sa);
+            }
+            if constexpr (S == 2)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const v8i av = fragment(i, 1, m);
+                    const uint32_t sa = scale(i, 1, m);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) acc[m][t] = tf_mx_product<FP4A, 1>(wv[i][1][t], av, acc[m][t], sh[t], sa);
+                }
+        }
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const int whole = KS >> 1;                                                   // units of two k-steps
+    int u = kw;
+    if constexpr (UNITS == 2)
+        for (; u + KW < whole; u += 2 * KW) units(two, two, u);
+    for (; u < whole; u += KW) units(one, two, u);
+    if (u < KU) units(one, one, u);
+    __syncthreads();                                                             // the regions of the rows become those of the sums
     // lane (g, r16) of acc[m][t]: columns 16 tile + 4 g .. + 3 of token row 16 m + r16
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -174,7 +241,7 @@ __global__ void __launch_bounds__(NW == 1 ? 512 : 1024) tf_mx_stream(const MxArg
         if constexpr (GATED) {
             __syncthreads();
             constexpr int PIECES = COLS / 8;
-            for (int i = threadIdx.x; i < 16 * PIECES; i += blockDim.x) {
+            for (int i = threadIdx.x; i < 16 * PIECES; i += blockDim.x) {        // (16 columns: half a wave, no codes)
                 const int r = i / PIECES, piece = i % PIECES, at = row0 + 16 * m + r, col = blockIdx.x * COLS + piece * 8;
                 const float* from = s_h + r * (COLS + 4) + piece * 8;
                 u4v h;
@@ -185,26 +252,47 @@ __global__ void __launch_bounds__(NW == 1 ? 512 : 1024) tf_mx_stream(const MxArg
         }
     }
 }
-template <bool FP4A, bool GATED, int CT, int MT, int NW>
-inline int tf_mx_stream_go(const MxArgs& p, int kw, hipStream_t s) {
+template <bool FP4A, bool GATED, int CT, int MT, int NW, int WAVES>
+inline int tf_mx_stream_go(const MxArgs& p, hipStream_t s) {
     constexpr int T = GATED ? 2 * CT : CT, COLS = NW * CT * 16;
-    const int waves = kw * NW;
-    const size_t lds = (size_t)waves * T * 1024 + (GATED ? 16 * (COLS + 4) * 4 : 0);
+    const int units = ((p.k + 127) / 128 + 1) / 2, most = WAVES / NW, waves = (units < most ? units : most) * NW;
+    constexpr int UNITS = tf_mx_units(GATED), OWN = UNITS * 2 * MT * 16 * (FP4A ? 64 : 128);
+    const size_t sums = (size_t)waves * T * 1024 + (GATED ? 16 * (COLS + 4) * 4 : 0), rows = (size_t)waves * OWN, lds = sums > rows ? sums : rows;
     const dim3 grid((p.n + COLS - 1) / COLS, (p.rows + 16 * MT - 1) / (16 * MT));
-    tf_mx_stream<FP4A, GATED, CT, MT, NW><<<grid, waves * 64, lds, s>>>(p);
+    tf_mx_stream<FP4A, GATED, CT, MT, NW, WAVES><<<grid, waves * 64, lds, s>>>(p);
     return (int)hipGetLastError();
 }
-template <bool FP4A, bool GATED, int CT, int NW>
-inline int tf_mx_stream_rows(const MxArgs& p, int most, hipStream_t s) {
-    const int rounds = (p.k + 511) / 512, kw = rounds < most ? rounds : most;
-    if (p.rows <= 16) return tf_mx_stream_go<FP4A, GATED, CT, 1, NW>(p, kw, s);
-    if (p.rows <= 32) return tf_mx_stream_go<FP4A, GATED, CT, 2, NW>(p, kw, s);
-    return tf_mx_stream_go<FP4A, GATED, CT, 4, NW>(p, kw, s);
+// Codes of an activation that is in memory: 8 columns a lane.
+__global__ void __launch_bounds__(256) tf_mx_codes(MxArgs p, uint32_t items) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, per_row = (uint32_t)p.n >> 3;
+    const bool on = i < items;
+    const uint32_t at = on ? i : 0, row = at / per_row, piece = at - row * per_row;
+    const u4v h = reinterpret_cast<const u4v*>(p.act)[at];
+    p.act = nullptr;
+    tf_mx_store_activation(p, h, row, (int)piece * 8, on);
 }
+inline int tf_launch_mx_codes(const MxArgs& p, hipStream_t s) {
+    const uint32_t items = (uint32_t)p.rows * ((uint32_t)p.n >> 3);
+    tf_mx_codes<<<(items + 255) / 256, 256, 0, s>>>(p, items);
+    return (int)hipGetLastError();
+}
+// Few rows.  Columns a workgroup: 16 while 32 would leave CUs without one (4 rows x 4,096 x 4,096: 256 workgroups); a gated product's hold
+// whole blocks of its codes: 32, or 128 of blocks of 128 where the activation itself has nowhere to go.  With the activation in memory
+// those codes are a launch of their own behind 16 columns a workgroup (4 rows x 2,048 x 4,096: 16 workgroups 11.8 us, 128 and the second
+// launch 7.2 us).
 template <bool FP4A>
-inline int tf_launch_mx_stream(const MxArgs& p, bool gated, hipStream_t s) {
-    if (!gated) return tf_mx_stream_rows<FP4A, false, 2, 1>(p, 8, s);
-    // a workgroup's columns hold whole blocks of the activation's codes
-    if (p.out_block == 128) return tf_mx_stream_rows<FP4A, true, 2, 4>(p, 4, s);
-    return tf_mx_stream_rows<FP4A, true, 2, 1>(p, 8, s);
+inline int tf_launch_mx_stream(const MxArgs& p, bool gated, int cus, hipStream_t s) {
+    const bool wide = (p.n + 31) / 32 >= cus;
+    if (!gated) {
+        if (p.rows <= 16) return wide ? tf_mx_stream_go<FP4A, false, 2, 1, 1, 16>(p, s) : tf_mx_stream_go<FP4A, false, 1, 1, 1, 16>(p, s);
+        return wide ? tf_mx_stream_go<FP4A, false, 2, 2, 1, 8>(p, s) : tf_mx_stream_go<FP4A, false, 1, 2, 1, 8>(p, s);
+    }
+    if (p.codes == nullptr || (p.out_block == 128 && p.act != nullptr)) {
+        MxArgs first = p;
+        first.codes = first.scales = nullptr;
+        const int status = wide ? tf_mx_stream_go<FP4A, true, 2, 1, 1, 16>(first, s) : tf_mx_stream_go<FP4A, true, 1, 1, 1, 16>(first, s);
+        return status || p.codes == nullptr ? status : tf_launch_mx_codes(p, s);
+    }
+    if (p.out_block == 128) return tf_mx_stream_go<FP4A, true, 2, 1, 4, 16>(p, s);
+    return tf_mx_stream_go<FP4A, true, 2, 1, 1, 16>(p, s);
 }
