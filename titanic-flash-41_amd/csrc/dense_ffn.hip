@@ -14,12 +14,9 @@ int check_device(const Context& c) {
     return e != hipSuccess ? (int)e : device != c.device ? -1 : 0;
 }
 int type_bytes(int type) { return type == CA_TYPE_FP32 ? 4 : 2; }
-// Items of eight values and workgroups of the byte-work kernels.
+// The byte-work kernels' items of eight values.
 constexpr long long kMaxItems = 0x7fffffffll;
-int byte_work_grid(const Context& c, long long items) {
-    const long long blocks = (items + 255) / 256, most = (long long)c.cus * 16;
-    return (int)(blocks < most ? blocks : most);
-}
+unsigned byte_work_grid(long long items) { return (unsigned)((items + 256 * TF_MXFP4_ITEMS - 1) / (256 * TF_MXFP4_ITEMS)); }
 int check_weights(int n, int k) { return n < 1 || n > (1 << 24) || k < 32 || k > 65536 || k % 32 ? -1 : 0; }
 int check_rows(const Context& c, int rows, int k, const void* a, const void* a_scales, int a_type) {
     if (rows < 0 || rows > (1 << 22) || (a_type != CA_MX_E4M3 && a_type != CA_MX_E2M1) || (a_type == CA_MX_E4M3 && k % c.g.act_block)) return -1;
@@ -61,12 +58,12 @@ int ca_mxfp4_quant(void* context, int rows, int cols, const void* x, int64_t x_s
     const Context& c = *(const Context*)context;
     const int device = check_device(c);
     if (device) return device;
-    const int grid = byte_work_grid(c, items);
+    const unsigned grid = byte_work_grid(items), count = (uint32_t)items, per_row = (uint32_t)cols >> 3, inverse = (uint32_t)((1ull << 32) / per_row);
     const hipStream_t s = (hipStream_t)stream;
     const uint8_t* from = (const uint8_t*)x;
-    if (x_type == CA_TYPE_BF16) tf_mxfp4_quant<TF_TYPE_BF16><<<grid, 256, 0, s>>>(from, pitch, (uint32_t*)words, (uint8_t*)scales, (uint32_t)items, (uint32_t)cols >> 3);
-    else if (x_type == CA_TYPE_FP16) tf_mxfp4_quant<TF_TYPE_FP16><<<grid, 256, 0, s>>>(from, pitch, (uint32_t*)words, (uint8_t*)scales, (uint32_t)items, (uint32_t)cols >> 3);
-    else tf_mxfp4_quant<TF_TYPE_FP32><<<grid, 256, 0, s>>>(from, pitch, (uint32_t*)words, (uint8_t*)scales, (uint32_t)items, (uint32_t)cols >> 3);
+    if (x_type == CA_TYPE_BF16) tf_mxfp4_quant<TF_TYPE_BF16><<<grid, 256, 0, s>>>(from, pitch, (uint32_t*)words, (uint8_t*)scales, count, per_row, inverse);
+    else if (x_type == CA_TYPE_FP16) tf_mxfp4_quant<TF_TYPE_FP16><<<grid, 256, 0, s>>>(from, pitch, (uint32_t*)words, (uint8_t*)scales, count, per_row, inverse);
+    else tf_mxfp4_quant<TF_TYPE_FP32><<<grid, 256, 0, s>>>(from, pitch, (uint32_t*)words, (uint8_t*)scales, count, per_row, inverse);
     return (int)hipGetLastError();
 }
 int ca_mxfp4_dequant(void* context, int rows, int cols, const void* words, const void* scales, void* out, int64_t out_stride, int out_type, void* stream) {
@@ -77,12 +74,12 @@ int ca_mxfp4_dequant(void* context, int rows, int cols, const void* words, const
     const Context& c = *(const Context*)context;
     const int device = check_device(c);
     if (device) return device;
-    const int grid = byte_work_grid(c, items);
+    const unsigned grid = byte_work_grid(items), count = (uint32_t)items, per_row = (uint32_t)cols >> 3, inverse = (uint32_t)((1ull << 32) / per_row);
     const hipStream_t s = (hipStream_t)stream;
     uint8_t* to = (uint8_t*)out;
-    if (out_type == CA_TYPE_BF16) tf_mxfp4_dequant<TF_TYPE_BF16><<<grid, 256, 0, s>>>((const uint32_t*)words, (const uint8_t*)scales, to, pitch, (uint32_t)items, (uint32_t)cols >> 3);
-    else if (out_type == CA_TYPE_FP16) tf_mxfp4_dequant<TF_TYPE_FP16><<<grid, 256, 0, s>>>((const uint32_t*)words, (const uint8_t*)scales, to, pitch, (uint32_t)items, (uint32_t)cols >> 3);
-    else tf_mxfp4_dequant<TF_TYPE_FP32><<<grid, 256, 0, s>>>((const uint32_t*)words, (const uint8_t*)scales, to, pitch, (uint32_t)items, (uint32_t)cols >> 3);
+    if (out_type == CA_TYPE_BF16) tf_mxfp4_dequant<TF_TYPE_BF16><<<grid, 256, 0, s>>>((const uint32_t*)words, (const uint8_t*)scales, to, pitch, count, per_row, inverse);
+    else if (out_type == CA_TYPE_FP16) tf_mxfp4_dequant<TF_TYPE_FP16><<<grid, 256, 0, s>>>((const uint32_t*)words, (const uint8_t*)scales, to, pitch, count, per_row, inverse);
+    else tf_mxfp4_dequant<TF_TYPE_FP32><<<grid, 256, 0, s>>>((const uint32_t*)words, (const uint8_t*)scales, to, pitch, count, per_row, inverse);
     return (int)hipGetLastError();
 }
 

@@ -68,33 +68,61 @@ __device__ __forceinline__ float tf_e8m0(uint32_t e) {
     return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(e ? e << 23 : 0x00400000u);
 }
 
+// Row and place in the row of item q, q / per_row by its reciprocal (inverse = 2^32 / per_row rounded down, per_row > 1): the estimate is at
+// most one short for q < 2^31.
+__device__ __forceinline__ void tf_item_place(uint32_t q, uint32_t per_row, uint32_t inverse, uint32_t& row, uint32_t& at) {
+    row = __umulhi(q, inverse);
+    at = q - row * per_row;
+    if (at >= per_row) { ++row; at -= per_row; }
+}
 // x [rows][cols] (row pitch `stride` bytes) -> words [rows][cols / 2], scales [rows][cols / 32].  One item = 8 values a lane; four
-// adjacent lanes hold a block.  HBM-bound byte work: 2 (4) bytes read, 17/32 written a value.
+// adjacent lanes hold a block; a workgroup takes 1,024 items, a thread's four loads in flight together.  HBM-bound byte work: 2 (4)
+// bytes read, 17/32 written a value.
+#define TF_MXFP4_ITEMS 4
 template <int TYPE>
 __global__ void __launch_bounds__(256) tf_mxfp4_quant(const uint8_t* __restrict__ x, long long stride, uint32_t* __restrict__ words,
-                                                      uint8_t* __restrict__ scales, uint32_t items, uint32_t per_row) {
+                                                      uint8_t* __restrict__ scales, uint32_t items, uint32_t per_row, uint32_t inverse) {
     constexpr int BYTES = TYPE == TF_TYPE_FP32 ? 32 : 16;
-    const uint32_t step = gridDim.x * blockDim.x;
-    for (uint32_t q = blockIdx.x * blockDim.x + threadIdx.x; q < items; q += step) {       // items, step: multiples of four
-        const uint32_t row = q / per_row, at = q - row * per_row;
-        float v[8];
-        tf_load8<TYPE>(x + (long long)row * stride + (long long)at * BYTES, v);
-        const uint32_t amax = tf_quad_max_bits(tf_amax_bits8(v));
-        const uint32_t e = tf_mxfp4_scale(amax);
-        words[q] = tf_mxfp4_codes8(v, tf_mxfp4_inverse(amax, e));
-        if ((q & 3) == 0) scales[q >> 2] = (uint8_t)e;
+    const uint32_t first = blockIdx.x * (256 * TF_MXFP4_ITEMS) + threadIdx.x;
+    float v[TF_MXFP4_ITEMS][8];
+#pragma unroll
+    for (int i = 0; i < TF_MXFP4_ITEMS; ++i) {
+        const uint32_t q = min(first + 256 * i, items - 1);              // (items is a multiple of four: the quads stay whole)
+        uint32_t row, at;
+        tf_item_place(q, per_row, inverse, row, at);
+        tf_load8<TYPE>(x + (long long)row * stride + (long long)at * BYTES, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < TF_MXFP4_ITEMS; ++i) {
+        const uint32_t q = first + 256 * i;
+        const uint32_t amax = tf_quad_max_bits(tf_amax_bits8(v[i])), e = tf_mxfp4_scale(amax);
+        const uint32_t codes = tf_mxfp4_codes8(v[i], tf_mxfp4_inverse(amax, e));
+        if (q < items) {
+            words[q] = codes;
+            if ((q & 3) == 0) scales[q >> 2] = (uint8_t)e;
+        }
     }
 }
 // The values of the codes, rounded once to the output's type (exact wherever it holds them).
 template <int TYPE>
 __global__ void __launch_bounds__(256) tf_mxfp4_dequant(const uint32_t* __restrict__ words, const uint8_t* __restrict__ scales, uint8_t* __restrict__ out,
-                                                        long long stride, uint32_t items, uint32_t per_row) {
+                                                        long long stride, uint32_t items, uint32_t per_row, uint32_t inverse) {
     constexpr int BYTES = TYPE == TF_TYPE_FP32 ? 32 : 16;
-    const uint32_t step = gridDim.x * blockDim.x;
-    for (uint32_t q = blockIdx.x * blockDim.x + threadIdx.x; q < items; q += step) {
-        const uint32_t row = q / per_row, at = q - row * per_row;
-        const uint32_t w = words[q];
-        const float s = tf_e8m0(scales[q >> 2]);
+    const uint32_t first = blockIdx.x * (256 * TF_MXFP4_ITEMS) + threadIdx.x;
+    uint32_t codes[TF_MXFP4_ITEMS], exponent[TF_MXFP4_ITEMS];
+#pragma unroll
+    for (int i = 0; i < TF_MXFP4_ITEMS; ++i) {
+        const uint32_t q = min(first + 256 * i, items - 1);
+        codes[i] = words[q];
+        exponent[i] = scales[q >> 2];
+    }
+#pragma unroll
+    for (int i = 0; i < TF_MXFP4_ITEMS; ++i) {
+        const uint32_t q = first + 256 * i, w = codes[i];
+        if (q >= items) continue;
+        uint32_t row, at;
+        tf_item_place(q, per_row, inverse, row, at);
+        const float s = tf_e8m0(exponent[i]);
         float v[8];
 #define TF_PAIR(i) { const tf_f32x2 t = __builtin_bit_cast(tf_f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, i)); v[2 * i] = __fmul_rn(t[0], s); v[2 * i + 1] = __fmul_rn(t[1], s); }
         TF_PAIR(0) TF_PAIR(1) TF_PAIR(2) TF_PAIR(3)
