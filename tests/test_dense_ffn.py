@@ -487,9 +487,11 @@ def test_linear(gpu, kind, block, rows, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,block", [(0, 32), (0, 128), (1, 32)])
-@pytest.mark.parametrize("rows,n,k", [(1090, 2100, 416), (1090, 2100, 640), (1025, 2304, 512), (4090, 4090, 512), (4090, 4090, 640), (4090, 4084, 544)])
+@pytest.mark.parametrize("rows,n,k", [(1090, 2100, 416), (1090, 2100, 640), (1025, 2304, 512), (4090, 4090, 512), (4090, 4090, 640), (4090, 4084, 544),
+                                       (4090, 4088, 512), (8190, 4088, 640), (8190, 4088, 1536)])
 def test_linear_large_tiles(gpu, kind, block, rows, n, k):
-    """Enough tiles that the larger ones are chosen, ragged in both directions.  The reference runs on the device in float64."""
+    """Enough tiles that the larger ones are chosen, and more than one a compute unit, ragged in both directions.  The reference runs on the
+    device in float64."""
     g = gpu(block)
     if block == 128:
         k = -(-k // 128) * 128
@@ -499,6 +501,11 @@ def test_linear_large_tiles(gpu, kind, block, rows, n, k):
     out = g.linear(rows, n, k, a, a_scales, kind, g.prepare(words, scales)).double()
     want, bound = device_product(av, wv, kind)
     assert bool(((out - want).abs() <= want.abs() * 2.0 ** -8 + bound).all())
+    # rows further apart: the same bits, nothing between the rows written
+    wide = g.guarded(rows, n + 8, dtype=torch.bfloat16)
+    g.linear(rows, n, k, a, a_scales, kind, g.prepare(words, scales), out=wide[:, :n])
+    g.check(wide)
+    assert torch.equal(wide[:, :n].double(), out) and bool((wide[:, n:].contiguous().view(torch.uint8) == 0xA5).all())
 
 
 def device_product(av, wv, kind):

@@ -43,27 +43,23 @@ __device__ __forceinline__ uint32_t tf_mx_lds(const void* p) { return (uint32_t)
 template <bool FP4A> struct MxFragment { typedef v8i type; };
 template <> struct MxFragment<true> { typedef u4v type; };
 // acc += weights x tokens, the sums held in place in the accumulator registers (256 of them leave the ordinary ones to the operands).
-// Lane (g, r) of the result: weight rows 4 g .. 4 g + 3 of the tile for token row r.  Read only behind tf_mx_settle().
-template <int SW, int ST>
+// Lane (g, r) of the result: weight rows 4 g .. 4 g + 3 of the tile for token row r.  The compiler does not know that these registers are
+// written late (12 wait states behind the instruction): wherever it may copy them, which is at the ends of its blocks, they have to be done.
+// So a k-step's LAST product waits 16 in the same statement, under the barrier that follows it.
+#define TF_MX_MFMA(FORMATS, WAIT) \
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] " FORMATS WAIT \
+                 : "+a"(acc) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(Q & 1), "n"(Q & 1), "n"(Q >> 1), "n"(Q >> 1))
+template <int Q, bool LAST>
 __device__ __forceinline__ void tf_mx_mfma(v4f& acc, const u4v& w, const v8i& a, uint32_t sw, uint32_t sa) {
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4"
-                 : "+a"(acc) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(SW & 1), "n"(ST & 1), "n"(SW >> 1), "n"(ST >> 1));
+    if constexpr (LAST) TF_MX_MFMA("cbsz:4", "\n\ts_nop 15");
+    else TF_MX_MFMA("cbsz:4", "");
 }
-template <int SW, int ST>
+template <int Q, bool LAST>
 __device__ __forceinline__ void tf_mx_mfma(v4f& acc, const u4v& w, const u4v& a, uint32_t sw, uint32_t sa) {
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
-                 : "+a"(acc) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(SW & 1), "n"(ST & 1), "n"(SW >> 1), "n"(ST >> 1));
+    if constexpr (LAST) TF_MX_MFMA("cbsz:4 blgp:4", "\n\ts_nop 15");
+    else TF_MX_MFMA("cbsz:4 blgp:4", "");
 }
-// The last results have reached the registers (the longest product takes 8 passes of 4 cycles), and the compiler reads none of these before.
-template <int FM, int FT>
-__device__ __forceinline__ void tf_mx_settle(v4f (&acc)[FM][FT]) {
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-        for (int t = 0; t < FT; t += 4) asm volatile("" : "+a"(acc[f][t]), "+a"(acc[f][t + 1]), "+a"(acc[f][t + 2]), "+a"(acc[f][t + 3]));
-}
-
+#undef TF_MX_MFMA
 // How a row's scales reach the lanes (all end as one register a fragment and round, byte q = k-step q of the round):
 enum { MX_SCALES_32 = 0,         // blocks of 32, k a multiple of 512: 16 bytes a row and round, copied by the memory system
        MX_SCALES_128 = 1,        // blocks of 128, k a multiple of 512: 4 bytes a row and round, likewise
@@ -74,6 +70,12 @@ enum { MX_SCALES_32 = 0,         // blocks of 32, k a multiple of 512: 16 bytes 
 // What the k-steps of the last round past the end of k multiply by: zero codes (a round is four k-steps whatever k is; the loop body then
 // has no branch, which its 256 accumulators would not survive in registers).
 static __device__ const u4v tf_mx_zeros[64] = {};
+
+// The largest tiles of a product of E2M1 rows: several a workgroup, one after the other, the next one's first k-steps on their way while the
+// last one's results are formed (16,384 x 4,096 x 2,048: 106 -> 87 us, 16,384 x 8,192 x 4,096: 370 -> 343).  E4M3 rows' operands leave too few registers
+// for it (4,096 x 4,096 x 4,096: 55 -> 57 us, 16,384 x 8,192 x 4,096: 486 -> 473), and a gated product's results spill beside them (16,384 x 8,192 x
+// 4,096: 945 -> 1,140).
+constexpr bool tf_mx_persistent(bool fp4_rows, bool gated, int products) { return fp4_rows && !gated && products == 64; }
 
 template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
 __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 16 ? 2 : 3) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
@@ -94,88 +96,101 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
 
     // Workgroup b runs on XCD b % 8.  An XCD takes a contiguous run of the tiles, eight row tiles side by side and column after column, so that the
     // tiles at work on it at once share their rows and weights in its L2.
-    const int total = tiles_m * tiles_n, chunk = (total + 7) >> 3;
-    const int id = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= chunk || id >= total) return;
-    const int band = id / (8 * tiles_n), in_band = id - band * 8 * tiles_n, band_m = min(8, tiles_m - band * 8);
-    const int tile_m = band * 8 + in_band % band_m, tile_n = in_band / band_m;
-    const int row0 = tile_m * BM, rows = min(BM, p.rows - row0);
+    constexpr bool PERSIST = tf_mx_persistent(FP4A, GATED, FM * FT);
+    const int total = tiles_m * tiles_n, chunk = (total + 7) >> 3, first_id = (blockIdx.x & 7) * chunk, last_id = min(first_id + chunk, total);
+    int id = first_id + (int)(blockIdx.x >> 3);
+    if (id >= last_id) return;
+    struct Tile { int row0, rows, n; };
+    auto tile_of = [&](int i) {
+        const int band = i / (8 * tiles_n), in_band = i - band * 8 * tiles_n, band_m = min(8, tiles_m - band * 8);
+        const int row0 = (band * 8 + in_band % band_m) * BM;
+        return Tile{row0, min(BM, p.rows - row0), in_band / band_m};
+    };
+    Tile cur = tile_of(id);
 
     // ---- requests ----------------------------------------------------------------------------------------------------
     const uint32_t lds_ring = tf_mx_lds(s_ring), lds_wsc = tf_mx_lds(s_wsc), lds_asc = tf_mx_lds(s_asc);
     // Every request is a scalar base that moves on with the k-step plus the lane's own offset; four requests share an m0, so a request's
     // offset holds 1,024 bytes for every one before it in its four less (and the bases point 4,096 bytes before their data).
     constexpr bool ROUNDS = SC <= MX_SCALES_128, STEPS = SC != MX_SCALES_ANY;   // k is whole rounds / k-steps: no request / no lane needs a bound
-    const uint8_t* a_base = p.a + (size_t)row0 * a_pitch - 4096;
-    uint32_t a_off[NA], a_col[NA];
+    const uint32_t lane16 = lane * 16;
+    uint32_t a_col[NA];
 #pragma unroll
     for (int c = 0; c < NA; ++c) {
-        const int row = (wave * NA + c) * ROWS_REQ + lane / LANES_ROW, r = row & 15;
+        const int r = ((wave * NA + c) * ROWS_REQ + lane / LANES_ROW) & 15;
         const int swz = FP4A ? ((r >> 1) & 3) ^ (r >> 3) : (r & 7) ^ (r >> 3);
         a_col[c] = (uint32_t)((lane % LANES_ROW) ^ swz) * 16;
-        // past the last row: that row again, never stored
-        a_off[c] = (uint32_t)min(row, rows - 1) * (uint32_t)a_pitch + 4096 - 1024 * (c & 3) + (STEPS ? a_col[c] : 0);
     }
-    // weight tile T of the workgroup (gated: a wave's FT tiles are FT / 2 of `up`, then the same columns' of `gate`)
-    auto weight_tile = [&](int T, bool& second) {
-        const int w = T / FT, t = T - w * FT;
-        second = GATED && t >= FT / 2;
-        const int tile = GATED ? tile_n * (TILES / 2) + w * (FT / 2) + (second ? t - FT / 2 : t) : tile_n * TILES + T;
-        return min(tile, n_tiles - 1);                                       // past the last tile: that tile again, never stored
-    };
     // the tiles a wave requests are of one matrix (gated: NB <= FT / 2), or half of them of either (NB == FT)
     constexpr bool BOTH = GATED && NB == FT;
     static_assert(!GATED || BOTH || FT / 2 % NB == 0, "whole halves");
-    const uint32_t lane16 = lane * 16;
-    const uint8_t* b_base[2];
-    uint32_t b_off[NB];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        bool second;
-        const int first = weight_tile(wave * NB + (BOTH ? half * (NB / 2) : 0), second);
-        b_base[half] = reinterpret_cast<const uint8_t*>(second ? p.w2 : p.w) + (size_t)first * KS * 1024 - 4096;
-#pragma unroll
-        for (int c = half * NB / 2; c < (half + 1) * NB / 2 || (NB == 1 && c == 0); ++c)
-            b_off[c] = (uint32_t)(weight_tile(wave * NB + c, second) - first) * (uint32_t)KS * 1024 + lane16 + 4096 - 1024 * (c & 3);
-    }
     // weight scales: a wave requests four tiles' 256 bytes of the round at once, 16 lanes a tile; waves past the tiles repeat the first ones' request
     const int wsc_wave = wave & (TILES / 4 - 1);
-    const uint8_t* wsc_base;
-    {
+    struct Source {                                                          // where a tile's requests come from
+        int row0, rows;
+        const uint8_t *a, *b[2], *wsc, *asc;                                 // (wsc, asc: the lane's own)
+        uint32_t a_off[NA], b_off[NB];
+    };
+    auto source_of = [&](const Tile& tile) {
+        Source s;
+        s.row0 = tile.row0; s.rows = tile.rows;
+        s.a = p.a + (size_t)tile.row0 * a_pitch - 4096;
+#pragma unroll
+        for (int c = 0; c < NA; ++c) {
+            const int row = (wave * NA + c) * ROWS_REQ + lane / LANES_ROW;
+            // past the last row: that row again, never stored
+            s.a_off[c] = (uint32_t)min(row, tile.rows - 1) * (uint32_t)a_pitch + 4096 - 1024 * (c & 3) + (STEPS ? a_col[c] : 0);
+        }
+        // weight tile T of the workgroup (gated: a wave's FT tiles are FT / 2 of `up`, then the same columns' of `gate`)
+        auto weight_tile = [&](int T, bool& second) {
+            const int w = T / FT, t = T - w * FT;
+            second = GATED && t >= FT / 2;
+            const int at = GATED ? tile.n * (TILES / 2) + w * (FT / 2) + (second ? t - FT / 2 : t) : tile.n * TILES + T;
+            return min(at, n_tiles - 1);                                     // past the last tile: that tile again, never stored
+        };
         bool second;
-        const int tile = weight_tile(wsc_wave * 4 + (lane >> 4), second);
-        wsc_base = reinterpret_cast<const uint8_t*>(second ? p.ws2 : p.ws) + (size_t)tile * KQ * 256 + (lane & 15) * 16;
-    }
-    const uint8_t* asc_row = p.a_scales + (size_t)(row0 + min(tid & (BM - 1), rows - 1)) * s_pitch;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int first = weight_tile(wave * NB + (BOTH ? half * (NB / 2) : 0), second);
+            s.b[half] = reinterpret_cast<const uint8_t*>(second ? p.w2 : p.w) + (size_t)first * KS * 1024 - 4096;
+#pragma unroll
+            for (int c = half * NB / 2; c < (half + 1) * NB / 2 || (NB == 1 && c == 0); ++c)
+                s.b_off[c] = (uint32_t)(weight_tile(wave * NB + c, second) - first) * (uint32_t)KS * 1024 + lane16 + 4096 - 1024 * (c & 3);
+        }
+        const int scale_tile = weight_tile(wsc_wave * 4 + (lane >> 4), second);
+        s.wsc = reinterpret_cast<const uint8_t*>(second ? p.ws2 : p.ws) + (size_t)scale_tile * KQ * 256 + (lane & 15) * 16;
+        s.asc = p.a_scales + (size_t)(tile.row0 + min(tid & (BM - 1), tile.rows - 1)) * s_pitch;
+        return s;
+    };
+    Source from = source_of(cur);
     const uint8_t* zeros = reinterpret_cast<const uint8_t*>(tf_mx_zeros) - 4096;
     // Request OP of k-step ks into the ring stage at lds_stage; the first of four sets m0.
     auto issue = [&](auto op_constant, int ks, uint32_t lds_stage) {
         constexpr int OP = decltype(op_constant)::value;
         if constexpr (OP < NA) {
             if constexpr (OP % 4 == 0) tf_mx_m0(lds_stage + (wave * NA + OP) * 1024);
-            if constexpr (STEPS) tf_mx_dma16<1024 * (OP & 3)>(a_base + (size_t)(ROUNDS ? ks : min(ks, KS - 1)) * ROWB, a_off[OP]);
-            else tf_mx_dma16<1024 * (OP & 3)>(a_base, a_off[OP] + min((uint32_t)ks * ROWB + a_col[OP], (uint32_t)a_pitch - 16));
+            if constexpr (STEPS) tf_mx_dma16<1024 * (OP & 3)>(from.a + (size_t)(ROUNDS ? ks : min(ks, KS - 1)) * ROWB, from.a_off[OP]);
+            else tf_mx_dma16<1024 * (OP & 3)>(from.a, from.a_off[OP] + min((uint32_t)ks * ROWB + a_col[OP], (uint32_t)a_pitch - 16));
         } else {
             constexpr int C = OP - NA, H = BOTH && C >= NB / 2 ? 1 : 0;
             if constexpr (C % 4 == 0) tf_mx_m0(lds_stage + A_STAGE + (wave * NB + C) * 1024);
-            if constexpr (ROUNDS) tf_mx_dma16<1024 * (C & 3)>(b_base[H] + (size_t)ks * 1024, b_off[C]);
-            else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? b_base[H] + (size_t)ks * 1024 : zeros, ks < KS ? b_off[C] : lane16 + 4096 - 1024 * (C & 3));
+            if constexpr (ROUNDS) tf_mx_dma16<1024 * (C & 3)>(from.b[H] + (size_t)ks * 1024, from.b_off[C]);
+            else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? from.b[H] + (size_t)ks * 1024 : zeros, ks < KS ? from.b_off[C] : lane16 + 4096 - 1024 * (C & 3));
         }
     };
     const int asc_wave = wave & (BM / 64 - 1);                               // waves past the tile's rows repeat the first ones' request
-    auto issue_scales = [&](int kq) {                                        // the MORE requests of a round (kq clamped: the count stays)
-        kq = min(kq, KQ - 1);
+    auto issue_scales = [&](int kq) {                                        // the MORE requests of a round
         tf_mx_m0(lds_wsc + wsc_wave * 1024);
-        tf_mx_dma16(wsc_base + (size_t)kq * 256);
-        if constexpr (SC == MX_SCALES_32) { tf_mx_m0(lds_asc + asc_wave * 1024); tf_mx_dma16(asc_row + kq * 16); }
-        if constexpr (SC == MX_SCALES_128) { tf_mx_m0(lds_asc + asc_wave * 256); tf_mx_dma4(asc_row + kq * 4); }
+        tf_mx_dma16(from.wsc + (size_t)kq * 256);
+        if constexpr (SC == MX_SCALES_32) { tf_mx_m0(lds_asc + asc_wave * 1024); tf_mx_dma16(from.asc + kq * 16); }
+        if constexpr (SC == MX_SCALES_128) { tf_mx_m0(lds_asc + asc_wave * 256); tf_mx_dma4(from.asc + kq * 4); }
         if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) {     // [k-step][row]
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int ks = min(4 * kq + q, KS - 1);
                 tf_mx_m0(lds_asc + q * (BM * 4) + asc_wave * 256);
-                if constexpr (SC == MX_SCALES_STEP_32) tf_mx_dma4(asc_row + ks * 4);
-                else tf_mx_dma1(asc_row + ks);
+                if constexpr (SC == MX_SCALES_STEP_32) tf_mx_dma4(from.asc + ks * 4);
+                else tf_mx_dma1(from.asc + ks);
             }
         }
         if constexpr (SC == MX_SCALES_ANY) {                                 // [block of the round][row]; request i of the wave's: block i / (BM / 64), 64 rows
@@ -183,7 +198,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
             for (int i = 0; i < MORE - 1; ++i) {
                 const int request = wave * (MORE - 1) + i, block = request / (BM / 64), row = request % (BM / 64) * 64;
                 tf_mx_m0(lds_asc + (block * BM + row) * 4);
-                tf_mx_dma1(p.a_scales + (size_t)(row0 + min(row + lane, rows - 1)) * s_pitch + min(16 * kq + block, s_pitch - 1));
+                tf_mx_dma1(p.a_scales + (size_t)(from.row0 + min(row + lane, from.rows - 1)) * s_pitch + min(16 * kq + block, s_pitch - 1));
             }
         }
     };
@@ -192,10 +207,6 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     const int swz = FP4A ? ((r16 >> 1) & 3) ^ (r16 >> 3) : (r16 & 7) ^ (r16 >> 3);
     const int a_at = (wm * 16 * FM + r16) * ROWB + ((g ^ swz) << 4), b_at = A_STAGE + wn * FT * 1024 + lane16;
     v4f acc[FM][FT];
-#pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-        for (int t = 0; t < FT; ++t) acc[f][t] = v4f{0.f, 0.f, 0.f, 0.f};
     Fragment av[2][FM];
     u4v wv[2][FT];
     uint32_t sa[2][FM], sw[2][FT];
@@ -235,19 +246,33 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     for (int f = 0; f < FM; ++f) { read_a(av[0][f], f, 0); read_sa(sa[0][f], f); }
 
     int stage = 0;                                                           // of k-step ks
+    // The k-step of a round that requests the next round's scales: the first from whose own requests on a persistent workgroup's last round asks
+    // for the next tile (k-step + NS lies past the round).
+    constexpr int SWITCH = 4 - NS;
     // requests that may be in flight at the top of k-step Q of a round: those of the NS - 2 k-steps before it
     auto behind = [](int q) constexpr {
         int n = 0;
-        for (int j = 1; j < NS - 1; ++j) n += DATA + (((q - j) & 3) == 0 ? MORE : 0);
+        for (int j = 1; j < NS - 1; ++j) n += DATA + (((q - j) & 3) == SWITCH ? MORE : 0);
         return n;
     };
-    auto k_step = [&](auto q_constant, int ks) {
+    Tile next = cur;
+    bool stored = false;                                                     // the tile before has stored: younger than the first k-steps' requests
+    auto k_step = [&](auto q_constant, int kq) {
         constexpr int Q = decltype(q_constant)::value, X = Q & 1, Y = X ^ 1;
-        const int next = NS == 4 ? (Q + 1) & 3 : (stage + 1 == NS ? 0 : stage + 1), now = NS == 4 ? Q : stage;
-        tf_mx_wait<behind(Q)>();
+        const int next_stage = NS == 4 ? (Q + 1) & 3 : (stage + 1 == NS ? 0 : stage + 1), now = NS == 4 ? Q : stage;
+        constexpr int STORES = FM * FT / 2;
+        static_assert(!PERSIST || behind(0) + STORES <= 63, "the counter's six bits");
+        if (PERSIST && Q < NS - 1 && kq == 0 && stored) tf_mx_wait<(PERSIST ? behind(Q) + STORES : 0)>();
+        else tf_mx_wait<behind(Q)>();
         tf_mx_barrier();
-        if constexpr (Q == 0) issue_scales((ks >> 2) + 1);
-        const int ahead = min(ks + NS, 4 * KQ - 1);                          // behind the last: that one again, never read
+        const bool last = kq == KQ - 1;
+        if constexpr (Q == SWITCH) {
+            if (PERSIST && last) from = source_of(next);
+            issue_scales(PERSIST ? (last ? 0 : kq + 1) : min(kq + 1, KQ - 1));       // (not persistent: the last round's again, never read)
+        }
+        int ahead = 4 * kq + Q + NS;                                         // behind the last k-step: the next tile's, or the last one again, never read
+        if constexpr (PERSIST) ahead = Q >= SWITCH && last ? Q - SWITCH : ahead;
+        else ahead = min(ahead, 4 * KQ - 1);
         const uint32_t lds_now = lds_ring + now * STAGE;
         // Product i (fragment i / FT, tile i % FT); behind it, spread over the step, what the next k-step needs from LDS (weights first) and the
         // requests, one instruction between two products where it fits: the wave is alone on its SIMD, and what does not issue under a
@@ -255,13 +280,13 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         constexpr int P = FM * FT, READS = FT + FM, SCALES = Q == 3 ? FT + FM : 0, ALL = READS + SCALES;
         tf_static_for<P>([&](auto i_constant) {
             constexpr int I = decltype(i_constant)::value, F = I / FT, T = I % FT;
-            tf_mx_mfma<Q, Q>(acc[F][T], wv[X][T], av[X][F], sw[0][T], sa[0][F]);
+            tf_mx_mfma<Q, I == P - 1>(acc[F][T], wv[X][T], av[X][F], sw[0][T], sa[0][F]);
             // reads within the first three quarters
             constexpr int R = I * ALL * 4 / (P * 3) < ALL ? I * ALL * 4 / (P * 3) : ALL, R_NEXT = (I + 1) * ALL * 4 / (P * 3) < ALL ? (I + 1) * ALL * 4 / (P * 3) : ALL;
             tf_static_for<R_NEXT - R>([&](auto j_constant) {
                 constexpr int J = R + decltype(j_constant)::value;
-                if constexpr (J < FT) read_w(wv[Y][J], J, next);
-                else if constexpr (J < READS) read_a(av[Y][J - FT], J - FT, next);
+                if constexpr (J < FT) read_w(wv[Y][J], J, next_stage);
+                else if constexpr (J < READS) read_a(av[Y][J - FT], J - FT, next_stage);
                 else if constexpr (J < READS + FT) read_sw(sw[1][J - READS], J - READS);
                 else read_sa(sa[1][J - READS - FT], J - READS - FT);
             });
@@ -269,20 +294,72 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
             tf_static_for<D_NEXT - D>([&](auto j_constant) { issue(std::integral_constant<int, D + decltype(j_constant)::value>{}, ahead, lds_now); });
             __builtin_amdgcn_sched_barrier(0);
         });
-        stage = next;
+        stage = next_stage;
     };
-    for (int kq = 0; kq < KQ; ++kq) {
-        k_step(std::integral_constant<int, 0>{}, 4 * kq);
-        k_step(std::integral_constant<int, 1>{}, 4 * kq + 1);
-        k_step(std::integral_constant<int, 2>{}, 4 * kq + 2);
-        k_step(std::integral_constant<int, 3>{}, 4 * kq + 3);
+    auto all_steps = [&]() {
 #pragma unroll
-        for (int f = 0; f < FM; ++f) sa[0][f] = sa[1][f];
+        for (int f = 0; f < FM; ++f)
 #pragma unroll
-        for (int t = 0; t < FT; ++t) sw[0][t] = sw[1][t];
+            for (int t = 0; t < FT; ++t) acc[f][t] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int kq = 0; kq < KQ; ++kq) {
+            k_step(std::integral_constant<int, 0>{}, kq);
+            k_step(std::integral_constant<int, 1>{}, kq);
+            k_step(std::integral_constant<int, 2>{}, kq);
+            k_step(std::integral_constant<int, 3>{}, kq);
+#pragma unroll
+            for (int f = 0; f < FM; ++f) sa[0][f] = sa[1][f];
+#pragma unroll
+            for (int t = 0; t < FT; ++t) sw[0][t] = sw[1][t];
+        }
+    };
+
+    if constexpr (PERSIST) {
+        // ---- tile after tile: while a tile's results are formed and stored, without LDS, the next one's first k-steps arrive in the ring ----------
+        const int per_xcd = gridDim.x >> 3;
+        for (;;) {
+            id += per_xcd;
+            const bool more = id < last_id;
+            if (more) next = tile_of(id);                                    // (else: the last tile's first k-steps again, never read)
+            all_steps();
+            // Two tiles' columns of a token row as BF16, eight consecutive ones a lane: lane group g takes tile t + g / 2, columns 8 (g % 2) ..; two
+            // swaps of lane rows a register pair instead of a way through LDS.
+            auto pieces = [](const v4f& first, const v4f& second) {
+                auto swapped = [](uint32_t a, uint32_t b) {
+                    const auto far = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+                    return __builtin_amdgcn_permlane16_swap(far[0], far[1], false, false);
+                };
+                const auto lo = swapped(tf_pack_bf16(first[0], first[1]), tf_pack_bf16(second[0], second[1]));
+                const auto hi = swapped(tf_pack_bf16(first[2], first[3]), tf_pack_bf16(second[2], second[3]));
+                return u4v{(uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1]};
+            };
+            // Every lane stores every time (a skipped store would make the count of the waits too high): what lies outside the tile goes to an
+            // offset past the descriptor's bytes, which the hardware drops.
+            constexpr uint32_t OUTSIDE = 0x80000000u;
+            auto bytes_at = [](void* base, size_t offset, size_t bytes) { return __builtin_amdgcn_make_buffer_rsrc((uint8_t*)base + offset, 0, (int)bytes, 0x00027000); };
+            const int first_row = wm * 16 * FM + r16, lane_col = (g >> 1) * 16 + (g & 1) * 8;
+            const auto to = bytes_at(p.out, (size_t)cur.row0 * p.out_stride * 2, ((size_t)(cur.rows - 1) * p.out_stride + p.n) * 2);
+            const int col0 = cur.n * COLS + wn * FT * 16 + lane_col;
+#pragma unroll
+            for (int f = 0; f < FM; ++f) {
+                const int row = first_row + 16 * f;
+                const uint32_t at = (uint32_t)(row * (int)p.out_stride + col0) * 2;
+#pragma unroll
+                for (int t = 0; t < FT; t += 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const u4v o = pieces(acc[f][t], acc[f][t + 1]);
+                    __builtin_amdgcn_raw_buffer_store_b128(o, to, row < cur.rows && col0 + t * 16 < p.n ? at + t * 32 : OUTSIDE, 0, 0);
+                }
+            }
+            stored = true;
+            if (!more) break;
+            cur = next;
+        }
+        tf_mx_wait<0>();                                                     // nothing is on its way into LDS any more
+        return;
     }
+    all_steps();
     tf_mx_wait<0>();                                                         // nothing writes LDS any more
-    tf_mx_settle(acc);
+    const int row0 = cur.row0, rows = cur.rows, tile_n = cur.n;
 
     // ---- results ---------------------------------------------------------------------------------------------------------
     // Lane (g, r16) of acc[f][t] holds columns 4 g .. 4 g + 3 of tile t for token row 16 f + r16 of the wave.  They pass through LDS as BF16 rows of
@@ -345,12 +422,13 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
 }
 
 template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
-inline int tf_mx_gemm_tiles(const MxArgs& p, hipStream_t s) {
+inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
     constexpr int ROWS = 16 * FM * WM, COLS = (GATED ? 8 : 16) * FT * WN;
     const int tiles_m = (p.rows + ROWS - 1) / ROWS, tiles_n = (p.n + COLS - 1) / COLS;
-    const long long total = (long long)tiles_m * tiles_n;
+    const long long total = (long long)tiles_m * tiles_n, whole = (total + 7) / 8 * 8, resident = cus / 8 * 8;
     if (total > 0x7ffffff0ll) return -1;
-    tf_mx_gemm<FP4A, GATED, SC, FM, FT, WM, WN, NS><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(p, tiles_m, tiles_n);
+    const long long grid = tf_mx_persistent(FP4A, GATED, FM * FT) && resident > 0 && resident < whole ? resident : whole;      // a workgroup a CU
+    tf_mx_gemm<FP4A, GATED, SC, FM, FT, WM, WN, NS><<<(unsigned)grid, 256, 0, s>>>(p, tiles_m, tiles_n);
     return (int)hipGetLastError();
 }
 // The tile's size.  A 256 x 256 tile takes 54 us of a CU at k = 4,096 (E4M3 rows), one of 128 x 128 (two a CU at once) 14.5 us, one of 64 x 64
@@ -362,29 +440,31 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, hipStream_t s) {
 // Blocks of 128 columns of a gated product's codes need the tile's columns to be whole blocks: 64 rows x 128 columns in place of the two
 // smaller ones, or, where 64 x 64 would be chosen and the activation goes to memory too, its codes in a launch of their own behind those
 // (64 rows x 2,048 x 4,096: 15.2 -> 9.6 us).
-inline int tf_mx_tile_size(const MxArgs& p, bool gated, int cus) {
+inline int tf_mx_tile_size(const MxArgs& p, bool fp4_rows, bool gated, int cus) {
     auto tiles = [&](int rows, int cols) { return (long long)((p.rows + rows - 1) / rows) * ((p.n * (gated ? 2ll : 1ll) + cols - 1) / cols); };
     auto rounds = [&](long long t) { return (t + cus - 1) / cus; };
     if (tiles(64, 64) <= 2 * cus) return 0;
+    // the persistent workgroups store whole 16-byte pieces, at 31-bit offsets from the tile's first row
+    if (tf_mx_persistent(fp4_rows, gated, 64) && (p.wide != 2 || p.n % 8 != 0 || p.out_stride > (1 << 21))) return 1;
     return 15 * rounds(tiles(256, 256)) <= 4 * rounds(tiles(128, 128)) ? 2 : 1;
 }
 template <bool FP4A, bool GATED, int SC>
 inline int tf_mx_gemm_go(const MxArgs& p, int cus, hipStream_t s) {
-    const int size = tf_mx_tile_size(p, GATED, cus);
+    const int size = tf_mx_tile_size(p, FP4A, GATED, cus);
     if constexpr (SC != MX_SCALES_ANY)
-        if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, s);
+        if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, cus, s);
     if constexpr (GATED)
         if (p.codes != nullptr && p.out_block == 128) {
             if (size == 0 && p.act != nullptr) {
                 MxArgs first = p;
                 first.codes = first.scales = nullptr;
-                const int status = tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(first, s);
+                const int status = tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(first, cus, s);
                 return status ? status : tf_launch_mx_codes(p, s);
             }
-            return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, s);
+            return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, cus, s);
         }
-    if (size >= 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, s);
-    return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, s);
+    if (size >= 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, cus, s);
+    return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, cus, s);
 }
 template <bool FP4A, bool GATED>
 inline int tf_launch_mx_gemm(const MxArgs& p, int cus, hipStream_t s) {
