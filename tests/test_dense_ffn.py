@@ -399,6 +399,9 @@ def test_add_norm_quant(gpu, block, rows, cols, pad, residual):
         again = res.clone() if pad == 0 else torch.nn.functional.pad(res, (0, pad))[:, :cols]
         g.norm(x, again, w, out=again, minimum=False)
         assert torch.equal(again, r)
+        again = x.clone() if pad == 0 else torch.nn.functional.pad(x, (0, pad))[:, :cols]
+        g.norm(again, res, w, out=again, minimum=False)
+        assert torch.equal(again, r)
 
 
 @pytest.mark.gpu
@@ -449,10 +452,10 @@ def product_error(a, w, kind):
     each cut off below 2^-13 of the power of two of the group's largest (measured on one product beside a large one: 2^-13 of it is kept, 2^-14
     is lost; 1.875 * 2^-11 of it comes back as 1.75 * 2^-11); the largest itself has six significant bits and loses nothing.  So seven products
     a group lose less than 2^-13 of max|a| max|w| each.  MXFP4 products span nine bits and lose nothing there.  The groups' sums and the
-    steps' meet in FP32; an addition is off by at most 2^-23 of its result (cut off), each partial sum is at most the sum of magnitudes,
-    and a term passes at most 16 additions: four levels of the instruction's 16 groups, the at most eight steps in a row of a
-    wave's rounds that matter against it, and the waves' join.  16 * 2^-23 = 2^-19."""
-    e = (np.abs(a) @ np.abs(w).T) * (2.0 ** -19)
+    steps' meet in FP32; an addition is off by at most 2^-23 of its result (cut off): four levels of the instruction's 16 groups, at most eight
+    additions where waves join, and the steps of 128 columns one after the other, whose partial sums grow from nothing to the
+    sum of magnitudes: half of k / 128 times it.  Together (16 + k / 256) 2^-23 of the sum of magnitudes."""
+    e = (np.abs(a) @ np.abs(w).T) * ((16 + a.shape[1] / 256) * 2.0 ** -23)
     if kind == native.MX_E4M3:
         most = lambda v: np.abs(v).reshape(v.shape[0], -1, 8).max(axis=2)
         e += (most(a) @ most(w).T) * (7 * 2.0 ** -13)
@@ -511,7 +514,7 @@ def test_linear_large_tiles(gpu, kind, block, rows, n, k):
 def device_product(av, wv, kind):
     """The product and product_error() on the device, in float64."""
     a, w = torch.from_numpy(av).cuda(), torch.from_numpy(wv).cuda()
-    e = (a.abs() @ w.abs().t().contiguous()) * 2.0 ** -19
+    e = (a.abs() @ w.abs().t().contiguous()) * ((16 + av.shape[1] / 256) * 2.0 ** -23)
     if kind == native.MX_E4M3:
         most = lambda v: v.abs().reshape(v.shape[0], -1, 8).amax(dim=2)
         e += (most(a) @ most(w).t().contiguous()) * (7 * 2.0 ** -13)
@@ -798,6 +801,42 @@ def test_refusals_on_a_real_context(gpu, block):
     for want, name, args in refusals(g.handle, block):
         assert getattr(g.lib, name)(*args) == want, (name, args)
     assert torch.cuda.is_available() and int(torch.ones(3, device="cuda").sum()) == 3      # no error was left behind
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("rows,n", [(3, 5), (300, 72)])
+def test_the_longest_contraction(gpu, kind, rows, n):
+    g = gpu(32)
+    k = 65536
+    a, a_scales, av = activations(g, kind, rows, k)
+    words, scales = mxfp4("long", n, k)
+    wv = values4(words, scales)
+    out = g.linear(rows, n, k, a, a_scales, kind, g.prepare(words, scales))
+    want = av @ wv.T
+    assert np.all(np.abs(f64(out) - want) <= np.abs(want) * 2.0 ** -8 + product_error(av, wv, kind))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(1, 1 << 24), (33, 1 << 24), (1 << 22, 16)])
+def test_the_largest_counts(gpu, rows, n):
+    """As many output columns, and rows, as a call may have: sampled ones against float64."""
+    g, k = gpu(32), 32
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    words = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    scales = torch.randint(120, 124, (n, 1), dtype=torch.uint8, device="cuda", generator=gen)
+    a = torch.randint(0, 0x70, (rows, k), dtype=torch.uint8, device="cuda", generator=gen)          # finite E4M3 codes
+    a_scales = torch.full((rows, 1), 120, dtype=torch.uint8, device="cuda")
+    w, ws = (torch.empty(size, dtype=torch.uint8, device="cuda") for size in (g.lib.ca_mxfp4_words_bytes(n, k), g.lib.ca_mxfp4_scales_bytes(n, k)))
+    p = native.ptr
+    assert g.lib.ca_mxfp4_prepare(g.ctx, n, k, p(words), p(scales), p(w), p(ws), g.stream()) == 0
+    out = torch.empty((rows, n), dtype=torch.bfloat16, device="cuda")
+    g.linear(rows, n, k, a, a_scales, 0, (w, ws), out=out)
+    r = torch.tensor(sorted({0, 1, rows // 2, rows - 2, rows - 1} & set(range(rows))))
+    c = torch.cat([torch.arange(min(n, 40)), torch.randint(0, n, (200,), generator=torch.Generator().manual_seed(1)), torch.arange(n - min(n, 40), n)])
+    av, wv = values8(a[r.cuda()], a_scales[r.cuda()], 32), values4(words[c.cuda()], scales[c.cuda()])
+    got, want = f64(out[r.cuda()][:, c.cuda()]), av @ wv.T
+    assert np.all(np.abs(got - want) <= np.abs(want) * 2.0 ** -8 + product_error(av, wv, 0))
 
 
 @pytest.mark.gpu
