@@ -30,10 +30,10 @@ __device__ __forceinline__ v4f tf_mx_product(const u4v& w, const v8i& a, const v
     const v8i wv = v8i{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, a, c, 4, FP4A ? 4 : 0, Q, (int)scale_w, 0, (int)scale_a);
 }
-// The activation of one pair of sums.  Comparisons, not minima: a NaN stays one.
+// The activation of one pair of sums.  (The minimum and maximum that keep a NaN.)
 __device__ __forceinline__ float tf_mx_swiglu(float up, float gate, float limit) {
-    const float g = gate > limit ? limit : gate;
-    const float u = up > limit ? limit : up < -limit ? -limit : up;
+    const float g = __builtin_elementwise_minimum(gate, limit);
+    const float u = __builtin_elementwise_maximum(__builtin_elementwise_minimum(up, limit), -limit);
     return __fmul_rn(__fmul_rn(g, tf_logistic_fast(g)), u);
 }
 // Eight consecutive columns of the activation (BF16) per lane: the BF16 copy, the codes and the block's scale byte.  All lanes of
