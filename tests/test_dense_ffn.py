@@ -114,7 +114,7 @@ def refusals(ctx, block=32):
     swiglu = dict(context=ctx, rows=2, inter=256, k=256, a=P, s=P, t=0, u=P, us=P, g=P, gs=P, act=P, c=P, cs=P, ot=0, stream=None)
     out = []
     for name, base, changes in [
-        ("ca_ffn_add_norm_quant", norm, [dict(context=None), dict(rows=-1), dict(x=None), dict(w=None), dict(c=None), dict(s=None), dict(cm=P), dict(sm=P), dict(eps=-1.0),
+        ("ca_ffn_add_norm_quant", norm, [dict(context=None), dict(rows=-1), dict(rows=(1 << 22) + 1), dict(x=None), dict(w=None), dict(c=None), dict(s=None), dict(cm=P), dict(sm=P), dict(eps=-1.0),
                                          dict(eps=float("nan")), dict(xs=i64(248)), dict(xs=i64(260)), dict(rs=i64(255)), dict(rs=i64(12)), dict(ros=i64(1)), dict(ros=i64(257)),
                                          dict(x=P + 2), dict(r=Q + 8), dict(w=P + 4), dict(ro=P + 1), dict(n=P + 8), dict(c=P + 4), dict(cm=P + 4, sm=P),
                                          dict(n=None, c=None, s=None, ro=None)]),
@@ -122,7 +122,7 @@ def refusals(ctx, block=32):
                                    dict(xs=i64(63)), dict(xs=i64(68)), dict(x=P + 8), dict(w=P + 2), dict(xs=i64(66), t=2), dict(rows=2 ** 31 - 1, cols=64)]),
         ("ca_mxfp4_dequant", dequant, [dict(context=None), dict(rows=-1), dict(cols=0), dict(cols=33), dict(t=3), dict(t=-1), dict(o=None), dict(w=None), dict(s=None),
                                        dict(os=i64(32)), dict(os=i64(65)), dict(o=P + 8), dict(w=P + 1), dict(rows=2 ** 31 - 1)]),
-        ("ca_mxfp4_prepare", prep, [dict(context=None), dict(n=0), dict(n=-1), dict(k=0), dict(k=48), dict(k=65568), dict(w=None), dict(s=None), dict(pw=None), dict(ps=None),
+        ("ca_mxfp4_prepare", prep, [dict(context=None), dict(n=0), dict(n=-1), dict(k=0), dict(k=48), dict(k=65568), dict(n=(1 << 20) + 1, k=65536), dict(w=None), dict(s=None), dict(pw=None), dict(ps=None),
                                     dict(pw=P), dict(ps=P), dict(w=P + 8), dict(pw=Q + 8), dict(ps=Q + 2)]),
         ("ca_mxfp4_linear", linear, [dict(context=None), dict(rows=-1), dict(rows=(1 << 22) + 1), dict(n=0), dict(k=0), dict(k=16), dict(k=65568), dict(t=2), dict(t=-1), dict(a=None),
                                      dict(s=None), dict(w=None), dict(ws=None), dict(o=None), dict(os=i64(15)), dict(a=P + 8), dict(w=P + 8), dict(ws=P + 2), dict(o=P + 1)]
@@ -161,6 +161,7 @@ def test_prepared_sizes():
         tiles = -(-n // 16)
         assert lib.ca_mxfp4_words_bytes(n, k) == tiles * -(-k // 128) * 1024
         assert lib.ca_mxfp4_scales_bytes(n, k) == tiles * -(-k // 512) * 256
+    assert lib.ca_mxfp4_words_bytes((1 << 20) + 1, 65536) == -1 and lib.ca_mxfp4_scales_bytes((1 << 20) + 1, 65536) == -1
     # above 2^31 bytes
     assert lib.ca_mxfp4_words_bytes(1 << 20, 65536) == 65536 * 512 * 1024
 

@@ -17,9 +17,11 @@ int type_bytes(int type) { return type == CA_TYPE_FP32 ? 4 : 2; }
 // The byte-work kernels' items of eight values.
 constexpr long long kMaxItems = 0x7fffffffll;
 unsigned byte_work_grid(long long items) { return (unsigned)((items + 256 * TF_MXFP4_ITEMS - 1) / (256 * TF_MXFP4_ITEMS)); }
-int check_weights(int n, int k) { return n < 1 || n > (1 << 24) || k < 32 || k > 65536 || k % 32 ? -1 : 0; }
+// Sizes whose launches stay below 2^32 threads.
+constexpr int kMaxRows = 1 << 22;
+int check_weights(int n, int k) { return n < 1 || n > (1 << 24) || k < 32 || k > 65536 || k % 32 || (long long)n * k > 1ll << 36 ? -1 : 0; }
 int check_rows(const Context& c, int rows, int k, const void* a, const void* a_scales, int a_type) {
-    if (rows < 0 || rows > (1 << 22) || (a_type != CA_MX_E4M3 && a_type != CA_MX_E2M1) || (a_type == CA_MX_E4M3 && k % c.g.act_block)) return -1;
+    if (rows < 0 || rows > kMaxRows || (a_type != CA_MX_E4M3 && a_type != CA_MX_E2M1) || (a_type == CA_MX_E4M3 && k % c.g.act_block)) return -1;
     if (rows > 0 && (!a || !a_scales || !aligned(a, 16))) return -1;
     return 0;
 }
@@ -31,7 +33,7 @@ extern "C" {
 int ca_ffn_add_norm_quant(void* context, int rows, int cols, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                           const void* weight, float eps, void* residual_out, int64_t residual_out_stride, void* normed, void* codes, void* scales,
                           void* codes_min, void* scales_min, void* stream) {
-    if (!context || rows < 0 || (!codes != !scales) || (!codes_min != !scales_min) || !(eps >= 0.f)) return -1;
+    if (!context || rows < 0 || rows > kMaxRows || (!codes != !scales) || (!codes_min != !scales_min) || !(eps >= 0.f)) return -1;
     const Context& c = *(const Context*)context;
     if (cols < c.g.act_block || cols > 8192 || cols % c.g.act_block) return -4;
     if (rows == 0) return 0;
@@ -92,7 +94,6 @@ int ca_mxfp4_prepare(void* context, int n, int k, const void* words, const void*
     const int device = check_device(*(const Context*)context);
     if (device) return device;
     const long long chunks = ca_mxfp4_words_bytes(n, k) / 16, scale_words = ca_mxfp4_scales_bytes(n, k) / 4;
-    if ((chunks + 255) / 256 > kMaxItems) return -1;
     tf_mxfp4_prepare_words<<<(unsigned)((chunks + 255) / 256), 256, 0, (hipStream_t)stream>>>((const u4v*)words, (u4v*)prepared_words, n, k, chunks);
     tf_mxfp4_prepare_scales<<<(unsigned)((scale_words + 255) / 256), 256, 0, (hipStream_t)stream>>>((const uint8_t*)scales, (uint32_t*)prepared_scales, n, k, scale_words);
     return (int)hipGetLastError();

@@ -426,7 +426,7 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
     constexpr int ROWS = 16 * FM * WM, COLS = (GATED ? 8 : 16) * FT * WN;
     const int tiles_m = (p.rows + ROWS - 1) / ROWS, tiles_n = (p.n + COLS - 1) / COLS;
     const long long total = (long long)tiles_m * tiles_n, whole = (total + 7) / 8 * 8, resident = cus / 8 * 8;
-    if (total > 0x7ffffff0ll) return -1;
+    if (total > 0xfffff0ll) return -1;                                      // 2^32 threads a launch
     const long long grid = tf_mx_persistent(FP4A, GATED, FM * FT) && resident > 0 && resident < whole ? resident : whole;      // a workgroup a CU
     tf_mx_gemm<FP4A, GATED, SC, FM, FT, WM, WN, NS><<<(unsigned)grid, 256, 0, s>>>(p, tiles_m, tiles_n);
     return (int)hipGetLastError();
