@@ -282,7 +282,7 @@ inline int tf_launch_mx_codes(const MxArgs& p, hipStream_t s) {
 // launch 7.2 us).
 template <bool FP4A>
 inline int tf_launch_mx_stream(const MxArgs& p, bool gated, int cus, hipStream_t s) {
-    const bool wide = (p.n + 31) / 32 >= cus;
+    const bool wide = (p.n + 15) / 16 > cus;
     if (!gated) {
         if (p.rows <= 16) return wide ? tf_mx_stream_go<FP4A, false, 2, 1, 1, 16>(p, s) : tf_mx_stream_go<FP4A, false, 1, 1, 1, 16>(p, s);
         return wide ? tf_mx_stream_go<FP4A, false, 2, 2, 1, 8>(p, s) : tf_mx_stream_go<FP4A, false, 1, 2, 1, 8>(p, s);
