@@ -370,7 +370,10 @@ def norm_want(x, residual, weight, eps):
 @pytest.mark.gpu
 @pytest.mark.parametrize("block", [32, 128])
 @pytest.mark.parametrize("rows,cols,pad,residual", [(1, 128, 0, True), (3, 384, 8, True), (5, 512, 0, False), (9, 640, 64, True), (7, 1024, 0, True), (6, 1152, 8, True),
-                                                    (5, 2048, 0, True), (4, 2176, 0, True), (33, 4096, 0, True), (3, 4224, 128, True), (17, 5120, 0, True), (2, 8192, 8, True)])
+                                                    (5, 2048, 0, True), (4, 2176, 0, True), (33, 4096, 0, True), (3, 4224, 128, True), (17, 5120, 0, True), (2, 8192, 8, True),
+                                                    # many rows
+                                                    (515, 640, 8, True), (514, 1024, 0, False), (530, 1152, 0, True), (600, 2048, 0, True), (515, 2176, 64, True),
+                                                    (513, 4096, 0, True), (530, 4224, 0, True), (520, 8192, 0, True)])
 def test_add_norm_quant(gpu, block, rows, cols, pad, residual):
     g = gpu(block)
     x = normal("norm/x", rows, cols + pad).to(torch.bfloat16).cuda()[:, :cols]

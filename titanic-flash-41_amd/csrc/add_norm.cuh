@@ -17,34 +17,40 @@ struct AddNormArgs {
     float eps;
 };
 
-// WAVES waves a row (1: four rows a workgroup; 4: one row a workgroup), PIECES 8-value pieces a lane.
+// WAVES waves a row (1: four rows a workgroup; else one), PIECES 8-value pieces a lane.
 template <int WAVES, int PIECES>
-__global__ void __launch_bounds__(256) tf_add_norm_quant(const AddNormArgs p) {
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_quant(const AddNormArgs p) {
     constexpr int LANES = WAVES * 64;
-    __shared__ float s_wave[4];
+    __shared__ float s_wave[WAVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int row = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     if (row >= p.rows) return;                             // a whole wave (WAVES 1: no barrier below) or nobody
     const int t = WAVES == 1 ? lane : threadIdx.x, per_row = p.cols >> 3, group_lanes = p.act_block >> 3;
     const u4v* x = reinterpret_cast<const u4v*>(p.x + (long long)row * p.x_stride);
     const u4v* res = reinterpret_cast<const u4v*>(p.residual + (long long)row * p.residual_stride);
+    const u4v* weight = reinterpret_cast<const u4v*>(p.weight);
     u4v* res_out = reinterpret_cast<u4v*>(p.residual_out + (long long)row * p.residual_out_stride);
-    u4v r[PIECES];
+    // Everything the row reads is requested before anything waits: with the loads inside `q < per_row` every piece was a round trip of its own.
+    u4v r[PIECES], b[PIECES], w[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) r[i] = x[min(i * LANES + t, per_row - 1)];
+    if (p.residual != nullptr)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) b[i] = res[min(i * LANES + t, per_row - 1)];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) w[i] = weight[min(i * LANES + t, per_row - 1)];
+    if (p.residual != nullptr)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                r[i][j] = tf_pack_bf16(__fadd_rn(tf_bf16_lo(r[i][j]), tf_bf16_lo(b[i][j])), __fadd_rn(tf_bf16_hi(r[i][j]), tf_bf16_hi(b[i][j])));
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int q = i * LANES + t;
-        r[i] = u4v{0, 0, 0, 0};
-        if (q < per_row) {
-            r[i] = x[q];
-            if (p.residual != nullptr) {
-                const u4v b = res[q];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    r[i][j] = tf_pack_bf16(__fadd_rn(tf_bf16_lo(r[i][j]), tf_bf16_lo(b[j])), __fadd_rn(tf_bf16_hi(r[i][j]), tf_bf16_hi(b[j])));
-            }
-            if (p.residual_out != nullptr) res_out[q] = r[i];
-        }
+        if (q >= per_row) r[i] = u4v{0, 0, 0, 0};
+        else if (p.residual_out != nullptr) res_out[q] = r[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             ss = __fmaf_rn(tf_bf16_lo(r[i][j]), tf_bf16_lo(r[i][j]), ss);
@@ -56,24 +62,22 @@ __global__ void __launch_bounds__(256) tf_add_norm_quant(const AddNormArgs p) {
     if constexpr (WAVES > 1) {
         if (lane == 0) s_wave[wave] = ss;
         __syncthreads();
-        ss = __fadd_rn(__fadd_rn(__fadd_rn(s_wave[0], s_wave[1]), s_wave[2]), s_wave[3]);
+        ss = s_wave[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) ss = __fadd_rn(ss, s_wave[i]);
     }
     const float inverse = 1.0f / __builtin_sqrtf(__fadd_rn(ss / (float)p.cols, p.eps));
-    const u4v* weight = reinterpret_cast<const u4v*>(p.weight);
     const int groups = p.cols / p.act_block;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int q = i * LANES + t;
         const bool on = q < per_row;                       // whole groups of lanes together: per_row is a multiple of group_lanes
         float v[8];
-        u4v o = {0, 0, 0, 0};
-        if (on) {
-            const u4v w = weight[q];
+        u4v o;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                o[j] = tf_pack_bf16(__fmul_rn(__fmul_rn(tf_bf16_lo(r[i][j]), inverse), tf_bf16_lo(w[j])),
-                                    __fmul_rn(__fmul_rn(tf_bf16_hi(r[i][j]), inverse), tf_bf16_hi(w[j])));
-        }
+        for (int j = 0; j < 4; ++j)
+            o[j] = tf_pack_bf16(__fmul_rn(__fmul_rn(tf_bf16_lo(r[i][j]), inverse), tf_bf16_lo(w[i][j])),
+                                __fmul_rn(__fmul_rn(tf_bf16_hi(r[i][j]), inverse), tf_bf16_hi(w[i][j])));
 #pragma unroll
         for (int j = 0; j < 4; ++j) { v[2 * j] = tf_bf16_lo(o[j]); v[2 * j + 1] = tf_bf16_hi(o[j]); }
         const float amax = tf_group_amax(v, group_lanes);
@@ -93,12 +97,23 @@ __global__ void __launch_bounds__(256) tf_add_norm_quant(const AddNormArgs p) {
         }
     }
 }
-// One wave a row up to 2,048 columns (four pieces a lane, no exchange between waves), four waves beyond.
-inline void tf_launch_add_norm(const AddNormArgs& p, hipStream_t s) {
-    const int grid = p.cols <= 2048 ? (p.rows + 3) / 4 : p.rows;
-    if (p.cols <= 512) tf_add_norm_quant<1, 1><<<grid, 256, 0, s>>>(p);
-    else if (p.cols <= 1024) tf_add_norm_quant<1, 2><<<grid, 256, 0, s>>>(p);
-    else if (p.cols <= 2048) tf_add_norm_quant<1, 4><<<grid, 256, 0, s>>>(p);
-    else if (p.cols <= 4096) tf_add_norm_quant<4, 2><<<grid, 256, 0, s>>>(p);
-    else tf_add_norm_quant<4, 4><<<grid, 256, 0, s>>>(p);
+// Up to two rows a CU the latency of the row's own loads, sums and exchange is the time, so a lane takes one piece (4 rows x 1,024: 2.7 us against 3.3
+// of one wave with two pieces, x 4,096: 2.95 against 3.5 of four waves, x 8,192: 4.6 against 5.8; 512 rows x 4,096: 5.5 against 5.9).  Beyond, HBM
+// is: fewer waves that meet at a barrier and more loads in flight a lane (2,048 rows x 4,096: 14.2 of eight waves against 13.1, 16,384 x 5,120: 144
+// against 134 us = 5.65 TB/s of the 9 bytes a value that the row moves; 16,384 x 1,024: four waves 28, one 23.5; 16,384 x 4,096 with a wave a row
+// 117 against 106).  The order of the sum of squares follows the variant.
+inline void tf_launch_add_norm(const AddNormArgs& p, int cus, hipStream_t s) {
+    const int quarter = (p.rows + 3) / 4;
+    if (p.cols <= 512) tf_add_norm_quant<1, 1><<<quarter, 256, 0, s>>>(p);
+    else if (p.rows <= 2 * cus) {
+        if (p.cols <= 1024) tf_add_norm_quant<2, 1><<<p.rows, 128, 0, s>>>(p);
+        else if (p.cols <= 2048) tf_add_norm_quant<4, 1><<<p.rows, 256, 0, s>>>(p);
+        else if (p.cols <= 4096) tf_add_norm_quant<8, 1><<<p.rows, 512, 0, s>>>(p);
+        else tf_add_norm_quant<16, 1><<<p.rows, 1024, 0, s>>>(p);
+    } else {
+        if (p.cols <= 1024) tf_add_norm_quant<1, 2><<<quarter, 256, 0, s>>>(p);
+        else if (p.cols <= 2048) tf_add_norm_quant<4, 1><<<p.rows, 256, 0, s>>>(p);
+        else if (p.cols <= 4096) tf_add_norm_quant<4, 2><<<p.rows, 256, 0, s>>>(p);
+        else tf_add_norm_quant<4, 4><<<p.rows, 256, 0, s>>>(p);
+    }
 }

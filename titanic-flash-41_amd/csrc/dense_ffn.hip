@@ -14,9 +14,9 @@ int check_device(const Context& c) {
     return e != hipSuccess ? (int)e : device != c.device ? -1 : 0;
 }
 int type_bytes(int type) { return type == CA_TYPE_FP32 ? 4 : 2; }
-// The byte-work kernels' items of eight values.
+// The byte-work kernels' items of eight values, one a thread.
 constexpr long long kMaxItems = 0x7fffffffll;
-unsigned byte_work_grid(long long items) { return (unsigned)((items + 256 * TF_MXFP4_ITEMS - 1) / (256 * TF_MXFP4_ITEMS)); }
+unsigned byte_work_grid(long long items) { return (unsigned)((items + 255) / 256); }
 // Sizes whose launches stay below 2^32 threads.
 constexpr int kMaxRows = 1 << 22;
 int check_weights(int n, int k) { return n < 1 || n > (1 << 24) || k < 32 || k > 65536 || k % 32 || (long long)n * k > 1ll << 36 ? -1 : 0; }
@@ -48,7 +48,7 @@ int ca_ffn_add_norm_quant(void* context, int rows, int cols, const void* x, int6
     if (device) return device;
     AddNormArgs p{(const uint16_t*)x, (const uint16_t*)residual, (const uint16_t*)weight, (uint16_t*)residual_out, (uint16_t*)normed, (uint8_t*)codes,
                   (uint8_t*)scales, (uint8_t*)codes_min, (uint8_t*)scales_min, x_stride, residual_stride, residual_out_stride, rows, cols, c.g.act_block, eps};
-    tf_launch_add_norm(p, (hipStream_t)stream);
+    tf_launch_add_norm(p, c.cus, (hipStream_t)stream);
     return (int)hipGetLastError();
 }
 

@@ -276,10 +276,10 @@ inline int tf_launch_mx_codes(const MxArgs& p, hipStream_t s) {
     tf_mx_codes<<<(items + 255) / 256, 256, 0, s>>>(p, items);
     return (int)hipGetLastError();
 }
-// Few rows.  Columns a workgroup: 16 while 32 would leave CUs without one (4 rows x 4,096 x 4,096: 256 workgroups); a gated product's hold
-// whole blocks of its codes: 32, or 128 of blocks of 128 where the activation itself has nowhere to go.  With the activation in memory
-// those codes are a launch of their own behind 16 columns a workgroup (4 rows x 2,048 x 4,096: 16 workgroups 11.8 us, 128 and the second
-// launch 7.2 us).
+// Few rows.  A workgroup fills a CU.  Columns a workgroup: 16 while that is one round of workgroups (4 rows x 4,096 x 4,096: 3.6 us against 4.0 of 32
+// columns), else 32 (16 rows x 5,120 x 4,096: 4.4 against 6.6, 32 rows x 8,192 x 8,192: 10.2 against 15.3).  A gated product's hold whole
+// blocks of its codes: 32, or 128 of blocks of 128 where the activation itself has nowhere to go.  With the activation in memory those codes
+// are a launch of their own behind 16 columns a workgroup (4 rows x 2,048 x 4,096: 16 workgroups 11.8 us, 128 and the second launch 7.2).
 template <bool FP4A>
 inline int tf_launch_mx_stream(const MxArgs& p, bool gated, int cus, hipStream_t s) {
     const bool wide = (p.n + 15) / 16 > cus;
