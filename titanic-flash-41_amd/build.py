@@ -1,7 +1,7 @@
 """Builds the package's native code in-tree with hipcc for gfx950.
 
   libtitanic_moe_hip.so      kernels + the C ABI of include/titanic_moe.h
-  titanic_moe_gfx950.hsaco   the same kernels as a code object for hosts that load modules by name
+  titanic_moe_gfx950.hsaco   the MoE layer's kernels as a code object for hosts that load modules by name
   libtitanic_ffn_host.so     the C++ host mirror of the reference's Rust FFN operators (needs only the HIP runtime)
   tf_layer_probe             stand-alone driver of the layer for profilers (no Python in the process)
   manifest.json              SHA-256 of the libraries just built; the host mirror refuses a kernel library that differs from it
