@@ -81,13 +81,16 @@ template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
 __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 16 ? 2 : 3) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
     constexpr int WAVES = WM * WN, BM = 16 * FM * WM, TILES = FT * WN, ROWB = FP4A ? 64 : 128;
     constexpr int A_STAGE = BM * ROWB, B_STAGE = TILES * 1024, STAGE = A_STAGE + B_STAGE;
-    constexpr int NA = A_STAGE / 1024 / WAVES, NB = TILES / WAVES, DATA = NA + NB, MORE = SC == MX_SCALES_ANY ? 1 + BM / 4 / WAVES : SC >= MX_SCALES_STEP_32 ? 5 : 2;
+    constexpr int NA = A_STAGE / 1024 / WAVES > 0 ? A_STAGE / 1024 / WAVES : 1, NB = TILES / WAVES, DATA = NA + NB, SROWS = BM < 64 ? 64 : BM;
+    constexpr int A_WAVES = A_STAGE / 1024 / NA;                               // waves past them repeat the first ones' requests of token rows
+    constexpr int MORE = SC == MX_SCALES_ANY ? 1 + SROWS / 4 / WAVES : SC >= MX_SCALES_STEP_32 ? 5 : 2;
     constexpr int COLS = (GATED ? TILES / 2 : TILES) * 16, LANES_ROW = ROWB / 16, ROWS_REQ = 64 / LANES_ROW;
-    static_assert(NA * WAVES * 1024 == A_STAGE && NB * WAVES == TILES && TILES % 4 == 0 && TILES <= 4 * WAVES && BM % 64 == 0 && BM <= WAVES * 64, "whole requests a wave");
+    static_assert(NA * A_WAVES * 1024 == A_STAGE && (A_WAVES & (A_WAVES - 1)) == 0 && A_WAVES <= WAVES && NB * WAVES == TILES && TILES % 4 == 0 && TILES <= 4 * WAVES &&
+                  SROWS % 64 == 0 && SROWS <= WAVES * 64, "whole requests a wave");
     typedef typename MxFragment<FP4A>::type Fragment;
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NS * STAGE];
     __shared__ __attribute__((aligned(1024))) uint32_t s_wsc[TILES * 64];
-    __shared__ __attribute__((aligned(1024))) uint32_t s_asc[SC == MX_SCALES_128 ? BM : SC == MX_SCALES_ANY ? BM * 16 : BM * 4];
+    __shared__ __attribute__((aligned(1024))) uint32_t s_asc[SC == MX_SCALES_128 ? SROWS : SC == MX_SCALES_ANY ? SROWS * 16 : SROWS * 4];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, g = lane >> 4, r16 = lane & 15;
@@ -115,9 +118,10 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     constexpr bool ROUNDS = SC <= MX_SCALES_128, STEPS = SC != MX_SCALES_ANY;   // k is whole rounds / k-steps: no request / no lane needs a bound
     const uint32_t lane16 = lane * 16;
     uint32_t a_col[NA];
+    const int a_wave = wave & (A_WAVES - 1);
 #pragma unroll
     for (int c = 0; c < NA; ++c) {
-        const int r = ((wave * NA + c) * ROWS_REQ + lane / LANES_ROW) & 15;
+        const int r = ((a_wave * NA + c) * ROWS_REQ + lane / LANES_ROW) & 15;
         const int swz = FP4A ? ((r >> 1) & 3) ^ (r >> 3) : (r & 7) ^ (r >> 3);
         a_col[c] = (uint32_t)((lane % LANES_ROW) ^ swz) * 16;
     }
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         s.a = p.a + (size_t)tile.row0 * a_pitch - 4096;
 #pragma unroll
         for (int c = 0; c < NA; ++c) {
-            const int row = (wave * NA + c) * ROWS_REQ + lane / LANES_ROW;
+            const int row = (a_wave * NA + c) * ROWS_REQ + lane / LANES_ROW;
             // past the last row: that row again, never stored
             s.a_off[c] = (uint32_t)min(row, tile.rows - 1) * (uint32_t)a_pitch + 4096 - 1024 * (c & 3) + (STEPS ? a_col[c] : 0);
         }
@@ -159,7 +163,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         }
         const int scale_tile = weight_tile(wsc_wave * 4 + (lane >> 4), second);
         s.wsc = reinterpret_cast<const uint8_t*>(second ? p.ws2 : p.ws) + (size_t)scale_tile * KQ * 256 + (lane & 15) * 16;
-        s.asc = p.a_scales + (size_t)(tile.row0 + min(tid & (BM - 1), tile.rows - 1)) * s_pitch;
+        s.asc = p.a_scales + (size_t)(tile.row0 + min(tid & (SROWS - 1), tile.rows - 1)) * s_pitch;
         return s;
     };
     Source from = source_of(cur);
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     auto issue = [&](auto op_constant, int ks, uint32_t lds_stage) {
         constexpr int OP = decltype(op_constant)::value;
         if constexpr (OP < NA) {
-            if constexpr (OP % 4 == 0) tf_mx_m0(lds_stage + (wave * NA + OP) * 1024);
+            if constexpr (OP % 4 == 0) tf_mx_m0(lds_stage + (a_wave * NA + OP) * 1024);
             if constexpr (STEPS) tf_mx_dma16<1024 * (OP & 3)>(from.a + (size_t)(ROUNDS ? ks : min(ks, KS - 1)) * ROWB, from.a_off[OP]);
             else tf_mx_dma16<1024 * (OP & 3)>(from.a, from.a_off[OP] + min((uint32_t)ks * ROWB + a_col[OP], (uint32_t)a_pitch - 16));
         } else {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
             else tf_mx_dma16<1024 * (C & 3)>(ks < KS ? from.b[H] + (size_t)ks * 1024 : zeros, ks < KS ? from.b_off[C] : lane16 + 4096 - 1024 * (C & 3));
         }
     };
-    const int asc_wave = wave & (BM / 64 - 1);                               // waves past the tile's rows repeat the first ones' request
+    const int asc_wave = wave & (SROWS / 64 - 1);                               // waves past the tile's rows repeat the first ones' request
     auto issue_scales = [&](int kq) {                                        // the MORE requests of a round
         tf_mx_m0(lds_wsc + wsc_wave * 1024);
         tf_mx_dma16(from.wsc + (size_t)kq * 256);
@@ -188,16 +192,16 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int ks = min(4 * kq + q, KS - 1);
-                tf_mx_m0(lds_asc + q * (BM * 4) + asc_wave * 256);
+                tf_mx_m0(lds_asc + q * (SROWS * 4) + asc_wave * 256);
                 if constexpr (SC == MX_SCALES_STEP_32) tf_mx_dma4(from.asc + ks * 4);
                 else tf_mx_dma1(from.asc + ks);
             }
         }
-        if constexpr (SC == MX_SCALES_ANY) {                                 // [block of the round][row]; request i of the wave's: block i / (BM / 64), 64 rows
+        if constexpr (SC == MX_SCALES_ANY) {                                 // [block of the round][row]; request i of the wave's: block i / (SROWS / 64), 64 rows
 #pragma unroll
             for (int i = 0; i < MORE - 1; ++i) {
-                const int request = wave * (MORE - 1) + i, block = request / (BM / 64), row = request % (BM / 64) * 64;
-                tf_mx_m0(lds_asc + (block * BM + row) * 4);
+                const int request = wave * (MORE - 1) + i, block = request / (SROWS / 64), row = request % (SROWS / 64) * 64;
+                tf_mx_m0(lds_asc + (block * SROWS + row) * 4);
                 tf_mx_dma1(p.a_scales + (size_t)(from.row0 + min(row + lane, from.rows - 1)) * s_pitch + min(16 * kq + block, s_pitch - 1));
             }
         }
@@ -224,8 +228,8 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
         if constexpr (SC == MX_SCALES_128) to = s_asc[row];
         else {                                                                // byte g of each k-step's word
             u4v w;
-            if constexpr (SC == MX_SCALES_ANY) w = u4v{s_asc[g * BM + row], s_asc[(4 + g) * BM + row], s_asc[(8 + g) * BM + row], s_asc[(12 + g) * BM + row]};
-            else if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) w = u4v{s_asc[row], s_asc[BM + row], s_asc[2 * BM + row], s_asc[3 * BM + row]};
+            if constexpr (SC == MX_SCALES_ANY) w = u4v{s_asc[g * SROWS + row], s_asc[(4 + g) * SROWS + row], s_asc[(8 + g) * SROWS + row], s_asc[(12 + g) * SROWS + row]};
+            else if constexpr (SC == MX_SCALES_STEP_32 || SC == MX_SCALES_STEP_128) w = u4v{s_asc[row], s_asc[SROWS + row], s_asc[2 * SROWS + row], s_asc[3 * SROWS + row]};
             else w = *reinterpret_cast<const u4v*>(s_asc + row * 4);
             const uint32_t byte = SC >= MX_SCALES_STEP_128 ? 0 : (uint32_t)g, pick = byte | ((4 + byte) << 8);       // of the second and the first operand
             const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], pick), hi = __builtin_amdgcn_perm(w[3], w[2], pick);
@@ -433,6 +437,7 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
 }
 // The tile's size.  A 256 x 256 tile takes 54 us of a CU at k = 4,096 (E4M3 rows), one of 128 x 128 (two a CU at once) 14.5 us, one of 64 x 64
 // 6 us (plus 3 us once): the large ones read LDS and L2 least for a product, the small ones give every CU something to do.
+//  - 32 x 64 while they are at most one a CU: 64 rows x 4,096: 6.8 us against 7.4 of 64 x 64, 64 rows x 8,192 x 8,192: 13.1, 15.1; 256 rows (two a CU): 9.4, 8.3
 //  - 64 x 64 while they are at most two a CU: 256 rows x 4,096: 8.5 us, against 14.8 (128) and 40 (256); 512 rows: 13.6, 15.8, 41
 //  - 256 x 256 where whole rounds of them cost less than whole rounds of 128 x 128, a quarter of the work at 15 / 16 of the time: 4,096 rows x
 //    4,096: 54 us against 58; but 2,048 rows (half the CUs without a tile) 46 against 30, 16 x 18 tiles (two rounds for 1.1) 74 against 70
@@ -443,10 +448,15 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
 inline int tf_mx_tile_size(const MxArgs& p, bool fp4_rows, bool gated, int cus) {
     auto tiles = [&](int rows, int cols) { return (long long)((p.rows + rows - 1) / rows) * ((p.n * (gated ? 2ll : 1ll) + cols - 1) / cols); };
     auto rounds = [&](long long t) { return (t + cus - 1) / cus; };
+    if (tiles(32, 64) <= cus) return -1;
     if (tiles(64, 64) <= 2 * cus) return 0;
     // the persistent workgroups store whole 16-byte pieces, at 31-bit offsets from the tile's first row
     if (tf_mx_persistent(fp4_rows, gated, 64) && (p.wide != 2 || p.n % 8 != 0 || p.out_stride > (1 << 21))) return 1;
     return 15 * rounds(tiles(256, 256)) <= 4 * rounds(tiles(128, 128)) ? 2 : 1;
+}
+template <bool FP4A, bool GATED, int SC>
+inline int tf_mx_gemm_small(const MxArgs& p, int size, int cus, hipStream_t s) {
+    return size < 0 ? tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 2, 2, 2, 4>(p, cus, s) : tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, cus, s);
 }
 template <bool FP4A, bool GATED, int SC>
 inline int tf_mx_gemm_go(const MxArgs& p, int cus, hipStream_t s) {
@@ -455,16 +465,16 @@ inline int tf_mx_gemm_go(const MxArgs& p, int cus, hipStream_t s) {
         if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, cus, s);
     if constexpr (GATED)
         if (p.codes != nullptr && p.out_block == 128) {
-            if (size == 0 && p.act != nullptr) {
+            if (size <= 0 && p.act != nullptr) {
                 MxArgs first = p;
                 first.codes = first.scales = nullptr;
-                const int status = tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(first, cus, s);
+                const int status = tf_mx_gemm_small<FP4A, GATED, SC>(first, size, cus, s);
                 return status ? status : tf_launch_mx_codes(p, s);
             }
             return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, cus, s);
         }
     if (size >= 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, cus, s);
-    return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, cus, s);
+    return tf_mx_gemm_small<FP4A, GATED, SC>(p, size, cus, s);
 }
 template <bool FP4A, bool GATED>
 inline int tf_launch_mx_gemm(const MxArgs& p, int cus, hipStream_t s) {
