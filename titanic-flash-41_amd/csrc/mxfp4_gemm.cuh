@@ -1,4 +1,4 @@
-// Products with prepared MXFP4 weights for many rows: tiles of 256 (128, 64) rows x as many weight rows on the matrix cores.
+// Products with prepared MXFP4 weights for many rows: tiles of 256 (128, 64) rows x as many weight rows, or 32 x 64, on the matrix cores.
 //
 // A workgroup of WM x WN = 4 waves (one a SIMD); a wave holds 16 FM token rows x 16 FT weight rows in 4 FM FT accumulator registers a lane.
 // A k-step is 128 columns: FM FT instructions of 16 x 16 x 128 a wave.  Both operands come into LDS by global_load_lds in a ring of NS
@@ -72,7 +72,7 @@ enum { MX_SCALES_32 = 0,         // blocks of 32, k a multiple of 512: 16 bytes 
 static __device__ const u4v tf_mx_zeros[64] = {};
 
 // The largest tiles of a product of E2M1 rows: several a workgroup, one after the other, the next one's first k-steps on their way while the
-// last one's results are formed (16,384 x 4,096 x 2,048: 106 -> 87 us, 16,384 x 8,192 x 4,096: 370 -> 343).  E4M3 rows' operands leave too few registers
+// last one's results are formed (16,384 x 4,096 x 2,048: 106 -> 87 us, 16,384 x 8,192 x 4,096: 314 -> 294).  E4M3 rows' operands leave too few registers
 // for it (4,096 x 4,096 x 4,096: 55 -> 57 us, 16,384 x 8,192 x 4,096: 486 -> 473), and a gated product's results spill beside them (16,384 x 8,192 x
 // 4,096: 945 -> 1,140).
 constexpr bool tf_mx_persistent(bool fp4_rows, bool gated, int products) { return fp4_rows && !gated && products == 64; }
@@ -444,7 +444,7 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
 //  - else 128 x 128: 1,024 rows: 18.8 us, against 25.5 (64) and 42 (256)
 // Blocks of 128 columns of a gated product's codes need the tile's columns to be whole blocks: 64 rows x 128 columns in place of the two
 // smaller ones, or, where 64 x 64 would be chosen and the activation goes to memory too, its codes in a launch of their own behind those
-// (64 rows x 2,048 x 4,096: 15.2 -> 9.6 us).
+// (64 rows x 2,048 x 4,096: 15.2 -> 9.0 us).
 inline int tf_mx_tile_size(const MxArgs& p, bool fp4_rows, bool gated, int cus) {
     auto tiles = [&](int rows, int cols) { return (long long)((p.rows + rows - 1) / rows) * ((p.n * (gated ? 2ll : 1ll) + cols - 1) / cols); };
     auto rounds = [&](long long t) { return (t + cus - 1) / cus; };
@@ -491,8 +491,8 @@ inline int tf_launch_mx_gemm(const MxArgs& p, int cus, hipStream_t s) {
     return -1;
 }
 // Both regimes of the products.  The streaming kernel reads every weight once for all its rows, but each workgroup reads all the rows: it takes
-// up to 32 (4,096 x 4,096: 24 rows 5.2 us against 6.9 of the 64 x 64 tiles, 40 rows 7.9 against 6.9), and 16 of a gated product, which has twice
-// the weights a column (2,048 x 4,096: 16 rows 6.2 us against 7.6, 24 rows 8.3 against 7.6).
+// up to 32 (4,096 x 4,096: 24 rows 5.2 us against 6.7 of the tiles, 40 rows 7.9 against 6.7), and 16 of a gated product, which has twice
+// the weights a column (2,048 x 4,096: 16 rows 6.2 us against 7.2, 24 rows 8.3 against 7.2).
 inline int tf_launch_mx(const MxArgs& p, bool gated, bool fp4_rows, int cus, hipStream_t s) {
     if (p.rows <= (gated ? 16 : 32)) return fp4_rows ? tf_launch_mx_stream<true>(p, gated, cus, s) : tf_launch_mx_stream<false>(p, gated, cus, s);
     if (gated) return fp4_rows ? tf_launch_mx_gemm<true, true>(p, cus, s) : tf_launch_mx_gemm<false, true>(p, cus, s);
