@@ -40,19 +40,35 @@ def _run(cmd):
 KERNEL_UNITS = ["abi.hip", "dense_ffn.hip"]
 
 
-def build_kernels():
-    def compile_unit(name, folder):
-        out = os.path.join(folder, name + ".o")
-        _run(["hipcc", *DEVICE_FLAGS, "-fPIC", "-c", os.path.join(CSRC, name), "-o", out])
-        return out
+def _compile(source, out, *flags):
+    """The compiler names a unit after its command line, paths included, unless it is given a name: with the file's own, the same sources give
+    the same bytes in whatever folder they lie and are built."""
+    unit = os.path.splitext(os.path.basename(source))[0]
+    _run(["hipcc", *DEVICE_FLAGS, "-cuid=" + unit, *flags, source, "-o", out])
+    return out
 
+
+def compile_unit(source, folder):
+    return _compile(source, os.path.join(folder, os.path.basename(source) + ".o"), "-fPIC", "-c")
+
+
+def compile_code_object(source, out):
+    return _compile(source, out, "--genco")
+
+
+def link_library(objects, library):
+    _run(["hipcc", "--offload-arch=gfx950", "-fPIC", "-shared", *objects, "-o", library])
+    return library
+
+
+def build_kernels():
     with tempfile.TemporaryDirectory() as folder, ThreadPoolExecutor(4) as pool:
-        units = [pool.submit(compile_unit, name, folder) for name in KERNEL_UNITS]
+        units = [pool.submit(compile_unit, os.path.join(CSRC, name), folder) for name in KERNEL_UNITS]
         objects = [
-            pool.submit(_run, ["hipcc", *DEVICE_FLAGS, "--genco", os.path.join(CSRC, "abi.hip"), "-o", CODE_OBJECT]),
+            pool.submit(compile_code_object, os.path.join(CSRC, "abi.hip"), CODE_OBJECT),
             # the kernels the reference launches by name with fixed argument lists, for its own layer's dimensions
-            pool.submit(_run, ["hipcc", *DEVICE_FLAGS, "--genco", os.path.join(CSRC, "reference_layer.hip"), "-o", REFERENCE_LAYER_OBJECT])]
-        _run(["hipcc", "--offload-arch=gfx950", "-fPIC", "-shared", *[u.result() for u in units], "-o", KERNEL_LIB])
+            pool.submit(compile_code_object, os.path.join(CSRC, "reference_layer.hip"), REFERENCE_LAYER_OBJECT)]
+        link_library([u.result() for u in units], KERNEL_LIB)
         for o in objects:
             o.result()
     return KERNEL_LIB
