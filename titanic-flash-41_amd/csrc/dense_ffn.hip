@@ -89,7 +89,7 @@ int64_t ca_mxfp4_words_bytes(int n, int k) { return check_weights(n, k) ? -1 : (
 int64_t ca_mxfp4_scales_bytes(int n, int k) { return check_weights(n, k) ? -1 : (int64_t)((n + 15) / 16) * ((k + 511) / 512) * 256; }
 int ca_mxfp4_prepare(void* context, int n, int k, const void* words, const void* scales, void* prepared_words, void* prepared_scales, void* stream) {
     if (!context || check_weights(n, k) || !words || !scales || !prepared_words || !prepared_scales || words == prepared_words || scales == prepared_scales ||
-        !aligned(words, 16) || !aligned(prepared_words, 16) || !aligned(prepared_scales, 4))
+        !aligned(words, 16) || !aligned(prepared_words, 16) || !aligned(prepared_scales, 16))
         return -1;
     const int device = check_device(*(const Context*)context);
     if (device) return device;
@@ -106,7 +106,7 @@ int ca_mxfp4_linear(void* context, int rows, int n, int k, const void* a, const 
     const int bad = check_rows(c, rows, k, a, a_scales, a_type);
     if (bad) return bad;
     if (rows == 0) return 0;
-    if (!w || !w_scales || !out || out_stride < n || !aligned(w, 16) || !aligned(w_scales, 4) || !aligned(out, 2)) return -1;
+    if (!w || !w_scales || !out || out_stride < n || !aligned(w, 16) || !aligned(w_scales, 16) || !aligned(out, 2)) return -1;
     const int device = check_device(c);
     if (device) return device;
     MxArgs p{};
@@ -123,8 +123,8 @@ int ca_mxfp4_swiglu(void* context, int rows, int inter, int k, const void* a, co
     const int bad = check_rows(c, rows, k, a, a_scales, a_type), block = out_type == CA_MX_E4M3 ? c.g.act_block : 32;
     if (bad || inter % block) return -1;
     if (rows == 0) return 0;
-    if (!up || !up_scales || !gate || !gate_scales || (!act && !codes) || !aligned(up, 16) || !aligned(gate, 16) || !aligned(up_scales, 4) ||
-        !aligned(gate_scales, 4) || !aligned(act, 16) || !aligned(codes, 8))
+    if (!up || !up_scales || !gate || !gate_scales || (!act && !codes) || !aligned(up, 16) || !aligned(gate, 16) || !aligned(up_scales, 16) ||
+        !aligned(gate_scales, 16) || !aligned(act, 16) || !aligned(codes, 8))
         return -1;
     const int device = check_device(c);
     if (device) return device;
