@@ -2,10 +2,25 @@
 sizes reach, results of a row in calls of different row counts.  References as in test_dense_ffn.py."""
 import ctypes
 
+import numpy as np
 import pytest
+import torch
 
 from helpers import native
-from test_dense_ffn import fake_context
+from test_dense_ffn import Gpu, f64, fake_context, norm_want, normal, quant8
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    made = {}
+
+    def get(block=32):
+        if block not in made:
+            made[block] = Gpu(block)
+        return made[block]
+    yield get
+    for g in made.values():
+        g.lib.ca_primitives_close(g.ctx)
 
 
 def test_scales_of_prepared_weights_lie_at_16_bytes():
@@ -18,3 +33,54 @@ def test_scales_of_prepared_weights_lie_at_16_bytes():
         assert lib.ca_mxfp4_linear(ctx, 64, 16, 256, P, P, 0, P, P + off, P, i64(16), None) == -1
         assert lib.ca_mxfp4_swiglu(ctx, 64, 256, 256, P, P, 0, P, P + off, P, P, P, P, P, 0, None) == -1
         assert lib.ca_mxfp4_swiglu(ctx, 64, 256, 256, P, P, 0, P, P, P, P + off, P, P, P, 0, None) == -1
+
+
+# ---- the norm's statistics --------------------------------------------------------------------------------------------------
+
+# every variant of waves and pieces a row, few rows and many
+NORM_SHAPES = [(9, 384), (9, 1024), (9, 2048), (9, 4096), (9, 8192), (520, 1024), (520, 4096), (520, 8192)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-6, 1e30])
+def test_norm_of_rows_whose_squares_leave_fp32(gpu, rows, cols, eps):
+    """Rows of every size that BF16 has: the squares of the large ones pass FP32's range, those of the small ones vanish in it (which shows where
+    eps is as small).  Each is the formula's value; the rows between are what they are alone."""
+    g = gpu(32)
+    x = normal("edges/norm", rows, cols).to(torch.float64)
+    sizes = [2.0 ** 125, 2.0 ** 100, 2.0 ** 66, 2.0 ** 61, 2.0 ** -40, 2.0 ** -62, 2.0 ** -80, 2.0 ** -110, 1.0]
+    x *= torch.tensor([sizes[i % len(sizes)] for i in range(rows)], dtype=torch.float64)[:, None]
+    x[0, 5], x[1, 7], x[1, 8] = 2.0 ** 127 * 1.5, 2.0 ** -126, 2.0 ** -60
+    x = x.to(torch.bfloat16).cuda()
+    w = (1.0 + normal("edges/norm-w", cols, std=0.2)).to(torch.bfloat16).cuda()
+    r, n, c, s, _, _ = g.norm(x, None, w, eps=eps, minimum=False)
+    assert torch.equal(r, x)
+    want = norm_want(x, None, w, float(np.float32(eps)))[1]
+    # Half a BF16 step (2^-134 where the result is subnormal) beside the FP32 chain of test_add_norm_quant, to which subnormal products add half of
+    # FP32's least value, 2^-150, each: the first times a weight below 2, and the second, less than 2^-148 in all.  The two add up: a value
+    # of 2^-134 (1 + 5.8e-6) comes out of the chain as the tie 2^-134, within 2^-149 of it, and goes to the even zero.
+    assert float(w.abs().max()) < 2
+    chain = np.abs(want) * (48 * 2.0 ** -24) + np.where(np.abs(want) < 2.0 ** -124, 2.0 ** -148, 0.0)
+    assert np.all(np.abs(f64(n) - want) <= np.maximum(np.abs(want) * 2.0 ** -8, 2.0 ** -134) + chain)
+    ordinary = np.abs(f64(n)).reshape(rows, -1, 32).max(axis=2).min(axis=1) > 2.0 ** -100      # (blocks below E4M3's scales have codes of their own)
+    codes, bytes_ = quant8(f64(n)[ordinary], 32)
+    assert ordinary[0] and np.array_equal(s.cpu().numpy()[ordinary], bytes_)
+    assert np.array_equal(c.cpu().view(torch.float8_e4m3fn).to(torch.float64).numpy()[ordinary], codes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+def test_norm_of_rows_that_are_not_finite(gpu, rows, cols):
+    """A NaN anywhere and an infinity at its own place stay NaN, and nothing else of the call changes; a sum past BF16's range is an infinity."""
+    g = gpu(32)
+    x = normal("edges/norm", rows, cols).to(torch.bfloat16).cuda()
+    res = normal("edges/norm-r", rows, cols).to(torch.bfloat16).cuda()
+    w = torch.ones(cols, dtype=torch.bfloat16, device="cuda")
+    clean = g.norm(x, res, w, minimum=False)
+    bad, other = x.clone(), res.clone()
+    bad[2, cols - 1], bad[4, 3], bad[6, 9], other[6, 9] = float("nan"), -float("inf"), 3e38, 3e38
+    r, n, c, s, _, _ = g.norm(bad, other, w, minimum=False)
+    keep = [i for i in range(rows) if i not in (2, 4, 6)]
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(clean[:4], (r, n, c, s)))
+    assert bool(torch.isnan(n[2]).all()) and bool(torch.isnan(n[4, 3])) and bool(torch.isinf(r[6, 9])) and bool(torch.isnan(n[6, 9]))

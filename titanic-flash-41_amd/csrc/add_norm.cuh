@@ -1,7 +1,8 @@
 // The boundary between two sublayers of a residual stream: the sublayer's output joins the residual, the sum is normalized and
 // quantized for the next product, in one pass over the row.
 //   r      = bf16(x + residual)                                       (residual == null: r = x)
-//   normed = bf16((r * (1 / sqrt(sum(r^2) / cols + eps))) * weight)     sum in FP32, division and root correctly rounded
+//   normed = bf16((r * (1 / sqrt(sum(r^2) / cols + eps))) * weight)     sum in FP32 (of a scaled row where FP32 does not hold it), division
+//                                                                       and root correctly rounded
 //   codes / scales (zero block: scale byte 0) and codes_min / scales_min (amax floored at 1e-4): the MXFP8 flavours of the normalized row,
 //   as ca_ffn_norm_quant has them
 // The statistics are those of the BF16 residual that the next boundary reads, so that they do not depend on who forms them.
@@ -57,16 +58,42 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_qua
             ss = __fmaf_rn(tf_bf16_hi(r[i][j]), tf_bf16_hi(r[i][j]), ss);
         }
     }
+    auto row_sum = [&](float v) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) ss = __fadd_rn(ss, __shfl_xor(ss, o));
-    if constexpr (WAVES > 1) {
-        if (lane == 0) s_wave[wave] = ss;
-        __syncthreads();
-        ss = s_wave[0];
+        for (int o = 1; o < 64; o <<= 1) v = __fadd_rn(v, __shfl_xor(v, o));
+        if constexpr (WAVES > 1) {
+            if (lane == 0) s_wave[wave] = v;
+            __syncthreads();
+            v = s_wave[0];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) ss = __fadd_rn(ss, s_wave[i]);
+            for (int i = 1; i < WAVES; ++i) v = __fadd_rn(v, s_wave[i]);
+        }
+        return v;
+    };
+    ss = row_sum(ss);
+    const float mean = __fadd_rn(ss / (float)p.cols, p.eps);
+    float inverse = 1.0f / __builtin_sqrtf(mean);
+    // Squares of BF16 values reach 2^256 and 2^-266.  Where their sum passes FP32's range, or is so small that squares of the row vanished in it, the
+    // row's statistics are formed again with the row scaled by a power of two: 2^-80 (its largest square is then 2^96) or 2^80 (the
+    // sum was below 2^-83, so the largest is 2^77, the least 2^-106).  1 / root is as small as 2^-128 for large rows, a subnormal: 2^8 of it goes to the row.
+    if (!(mean >= 0x1p-96f && mean < __builtin_inff())) {      // the whole row's lanes alike; NaN too, and comes out as NaN
+        const bool small = mean < 1.f;
+        const float scale = small ? 0x1p80f : 0x1p-80f, share = small ? 0x1p80f : 0x1p-8f;
+        ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float lo = tf_bf16_lo(r[i][j]), hi = tf_bf16_hi(r[i][j]), a = __fmul_rn(lo, scale), b = __fmul_rn(hi, scale);
+                ss = __fmaf_rn(a, a, ss);
+                ss = __fmaf_rn(b, b, ss);
+                r[i][j] = tf_pack_bf16(__fmul_rn(lo, share), __fmul_rn(hi, share));      // exact, or so small that its result is zero
+            }
+        if constexpr (WAVES > 1) __syncthreads();                                        // s_wave has been read
+        ss = row_sum(ss);
+        inverse = 1.0f / __builtin_sqrtf(__fadd_rn(ss / (float)p.cols, __fmul_rn(__fmul_rn(p.eps, scale), scale)));
+        if (!small) inverse = __fmul_rn(inverse, 0x1p-72f);
     }
-    const float inverse = 1.0f / __builtin_sqrtf(__fadd_rn(ss / (float)p.cols, p.eps));
     const int groups = p.cols / p.act_block;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
