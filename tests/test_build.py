@@ -1,6 +1,8 @@
 """The native build: the same sources give the same library."""
 import importlib
 
+import pytest
+
 build = importlib.import_module("titanic-flash-41_amd.build")
 
 # a unit with a device variable of its own file, whose symbol carries the unit's name
@@ -27,3 +29,22 @@ def test_the_library_does_not_depend_on_where_it_is_built(tmp_path):
 
 def test_units_have_names_of_their_own():
     assert len(set(build.KERNEL_UNITS)) == len(build.KERNEL_UNITS)
+
+
+def test_a_broken_promise_of_the_launch_bounds_fails_the_build(tmp_path):
+    """Two workgroups a CU of which one fills more than half of LDS."""
+    source = """#include <hip/hip_runtime.h>
+__global__ void __launch_bounds__(256, %d) kernel(int* p) {
+    __shared__ int s[100 * 256];
+    s[threadIdx.x * 97] = p[threadIdx.x];
+    __syncthreads();
+    p[threadIdx.x] = s[threadIdx.x];
+}
+"""
+    for promised in (1, 2):
+        (tmp_path / "unit.hip").write_text(source % promised)
+        if promised == 1:
+            build.compile_unit(str(tmp_path / "unit.hip"), str(tmp_path))
+        else:
+            with pytest.raises(RuntimeError, match="occupancy"):
+                build.compile_unit(str(tmp_path / "unit.hip"), str(tmp_path))

@@ -22,9 +22,10 @@ HOST_LIB = os.path.join(HERE, "libtitanic_ffn_host.so")
 PROBE = os.path.join(HERE, "tf_layer_probe")
 MANIFEST = os.path.join(HERE, "manifest.json")
 
-# -ffp-contract=off: bit-exact steps are written as explicit fma / mul / add.  Packed FP32 instructions stay off.
+# -ffp-contract=off: bit-exact steps are written as explicit fma / mul / add.  Packed FP32 instructions stay off.  A kernel that cannot have the
+# workgroups a CU that its launch bounds promise, or a loop that does not unroll as it is told to, is an error.
 DEVICE_FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang",
-                "-packed-fp32-ops", "-Wno-unused-command-line-argument"]
+                "-packed-fp32-ops", "-Wno-unused-command-line-argument", "-Werror=pass-failed"]
 
 
 def _run(cmd):

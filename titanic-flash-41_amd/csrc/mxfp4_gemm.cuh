@@ -77,11 +77,24 @@ static __device__ const u4v tf_mx_zeros[64] = {};
 // 4,096: 945 -> 1,140).
 constexpr bool tf_mx_persistent(bool fp4_rows, bool gated, int products) { return fp4_rows && !gated && products == 64; }
 
+// LDS of a workgroup: the ring, the weights' scales of a round, the rows' (a word a row and block where SC is MX_SCALES_ANY).
+constexpr int tf_mx_scale_rows(int fm, int wm) { return 16 * fm * wm < 64 ? 64 : 16 * fm * wm; }
+constexpr int tf_mx_scale_words(int sc, int rows) { return sc == MX_SCALES_128 ? rows : sc == MX_SCALES_ANY ? rows * 16 : rows * 4; }
+constexpr int tf_mx_lds_bytes(bool fp4_rows, int sc, int fm, int ft, int wm, int wn, int stages) {
+    return stages * (16 * fm * wm * (fp4_rows ? 64 : 128) + ft * wn * 1024) + ft * wn * 256 + tf_mx_scale_words(sc, tf_mx_scale_rows(fm, wm)) * 4;
+}
+// Workgroups a CU: as many as leave registers for the sums (the largest tiles 1, 64 sums a lane 2, else 3) and fit into its 160 KiB.  With 64 sums
+// it is 1 for the MX_SCALES_ANY tiles of 128 x 128 E4M3 rows (83,968 bytes) and for the gated 64 x 128 tiles of E2M1 rows (87,040 to 90,112).
+constexpr int tf_mx_resident(bool fp4_rows, int sc, int fm, int ft, int wm, int wn, int stages) {
+    const int registers = fm * ft >= 64 ? 1 : fm * ft >= 16 ? 2 : 3, lds = 160 * 1024 / tf_mx_lds_bytes(fp4_rows, sc, fm, ft, wm, wn, stages);
+    return registers < lds ? registers : lds;
+}
+
 template <bool FP4A, bool GATED, int SC, int FM, int FT, int WM, int WN, int NS>
-__global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 16 ? 2 : 3) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(WM * WN * 64, tf_mx_resident(FP4A, SC, FM, FT, WM, WN, NS)) tf_mx_gemm(const MxArgs p, int tiles_m, int tiles_n) {
     constexpr int WAVES = WM * WN, BM = 16 * FM * WM, TILES = FT * WN, ROWB = FP4A ? 64 : 128;
     constexpr int A_STAGE = BM * ROWB, B_STAGE = TILES * 1024, STAGE = A_STAGE + B_STAGE;
-    constexpr int NA = A_STAGE / 1024 / WAVES > 0 ? A_STAGE / 1024 / WAVES : 1, NB = TILES / WAVES, DATA = NA + NB, SROWS = BM < 64 ? 64 : BM;
+    constexpr int NA = A_STAGE / 1024 / WAVES > 0 ? A_STAGE / 1024 / WAVES : 1, NB = TILES / WAVES, DATA = NA + NB, SROWS = tf_mx_scale_rows(FM, WM);
     constexpr int A_WAVES = A_STAGE / 1024 / NA;                               // waves past them repeat the first ones' requests of token rows
     constexpr int MORE = SC == MX_SCALES_ANY ? 1 + SROWS / 4 / WAVES : SC >= MX_SCALES_STEP_32 ? 5 : 2;
     constexpr int COLS = (GATED ? TILES / 2 : TILES) * 16, LANES_ROW = ROWB / 16, ROWS_REQ = 64 / LANES_ROW;
@@ -90,7 +103,8 @@ __global__ void __launch_bounds__(WM * WN * 64, FM * FT >= 64 ? 1 : FM * FT >= 1
     typedef typename MxFragment<FP4A>::type Fragment;
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[NS * STAGE];
     __shared__ __attribute__((aligned(1024))) uint32_t s_wsc[TILES * 64];
-    __shared__ __attribute__((aligned(1024))) uint32_t s_asc[SC == MX_SCALES_128 ? SROWS : SC == MX_SCALES_ANY ? SROWS * 16 : SROWS * 4];
+    __shared__ __attribute__((aligned(1024))) uint32_t s_asc[tf_mx_scale_words(SC, SROWS)];
+    static_assert(sizeof(s_ring) + sizeof(s_wsc) + sizeof(s_asc) == tf_mx_lds_bytes(FP4A, SC, FM, FT, WM, WN, NS), "the LDS that the occupancy was counted with");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, g = lane >> 4, r16 = lane & 15;
@@ -442,6 +456,9 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
 //  - 256 x 256 where whole rounds of them cost less than whole rounds of 128 x 128, a quarter of the work at 15 / 16 of the time: 4,096 rows x
 //    4,096: 54 us against 58; but 2,048 rows (half the CUs without a tile) 46 against 30, 16 x 18 tiles (two rounds for 1.1) 74 against 70
 //  - else 128 x 128: 1,024 rows: 18.8 us, against 25.5 (64) and 42 (256)
+// All of these were taken with E4M3 rows at a k of 4,096; the rule stands unmeasured for E2M1 rows, gated products and other k.  It is known to be off where k is no
+// multiple of 128 with blocks of 32: no 256 x 256 tile has room for the scales, and of E4M3 rows' 128 x 128 one fits a CU instead of two (4,096 x
+// 4,096 x 4,128 88 us, x 4,224 57; E2M1 rows 62 and the gated 4,096 x 2,048 x 4,128 94).
 // Blocks of 128 columns of a gated product's codes need the tile's columns to be whole blocks: 64 rows x 128 columns in place of the two
 // smaller ones, or, where 64 x 64 would be chosen and the activation goes to memory too, its codes in a launch of their own behind those
 // (64 rows x 2,048 x 4,096: 15.2 -> 9.0 us).
