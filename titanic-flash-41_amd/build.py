@@ -6,6 +6,7 @@
   tf_layer_probe             stand-alone driver of the layer for profilers (no Python in the process)
   manifest.json              SHA-256 of the libraries just built; the host mirror refuses a kernel library that differs from it
 """
+import importlib
 import os
 import subprocess
 import tempfile
@@ -62,6 +63,12 @@ def link_library(objects, library):
     return library
 
 
+def check_products(path):
+    """The machine code of the many-row products against what their inline assembly relies on; RuntimeError where it does not hold."""
+    if not importlib.import_module("titanic-flash-41_amd.listing").check(path):
+        raise RuntimeError("%s holds no many-row products" % path)
+
+
 def build_kernels():
     with tempfile.TemporaryDirectory() as folder, ThreadPoolExecutor(4) as pool:
         units = [pool.submit(compile_unit, os.path.join(CSRC, name), folder) for name in KERNEL_UNITS]
@@ -70,6 +77,7 @@ def build_kernels():
             # the kernels the reference launches by name with fixed argument lists, for its own layer's dimensions
             pool.submit(compile_code_object, os.path.join(CSRC, "reference_layer.hip"), REFERENCE_LAYER_OBJECT)]
         link_library([u.result() for u in units], KERNEL_LIB)
+        check_products(KERNEL_LIB)
         for o in objects:
             o.result()
     return KERNEL_LIB
@@ -111,7 +119,6 @@ def write_manifest():
 def write_pinned_contracts():
     """The operator contracts with the hash of the library just built (contracts/pinned/, beside the committed ones, whose
     hash fields are null because no library is committed)."""
-    import importlib
     contracts = importlib.import_module("titanic-flash-41_amd.contracts")
     contracts.main(os.path.join(HERE, "contracts", "pinned"), KERNEL_LIB)
 

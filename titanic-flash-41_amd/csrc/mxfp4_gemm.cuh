@@ -45,7 +45,8 @@ template <> struct MxFragment<true> { typedef u4v type; };
 // acc += weights x tokens, the sums held in place in the accumulator registers (256 of them leave the ordinary ones to the operands).
 // Lane (g, r) of the result: weight rows 4 g .. 4 g + 3 of the tile for token row r.  The compiler does not know that these registers are
 // written late (12 wait states behind the instruction): wherever it may copy them, which is at the ends of its blocks, they have to be done.
-// So a k-step's LAST product waits 16 in the same statement, under the barrier that follows it.
+// So a k-step's LAST product waits 16 in the same statement, under the barrier that follows it.  The build reads the machine code and fails where it
+// touches a sum, an operand, a request's base or the count of requests in a way that these statements do not allow for (listing.py).
 #define TF_MX_MFMA(FORMATS, WAIT) \
     asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] " FORMATS WAIT \
                  : "+a"(acc) : "v"(w), "v"(a), "v"(sw), "v"(sa), "n"(Q & 1), "n"(Q & 1), "n"(Q >> 1), "n"(Q >> 1))
