@@ -61,22 +61,9 @@ __device__ __forceinline__ void tf_mx_mfma(v4f& acc, const u4v& w, const u4v& a,
     else TF_MX_MFMA("cbsz:4 blgp:4", "");
 }
 #undef TF_MX_MFMA
-// How a row's scales reach the lanes (all end as one register a fragment and round, byte q = k-step q of the round):
-enum { MX_SCALES_32 = 0,         // blocks of 32, k a multiple of 512: 16 bytes a row and round, copied by the memory system
-       MX_SCALES_128 = 1,        // blocks of 128, k a multiple of 512: 4 bytes a row and round, likewise
-       MX_SCALES_STEP_32 = 2,    // blocks of 32, k a multiple of 128: 4 bytes a row and k-step
-       MX_SCALES_STEP_128 = 3,   // blocks of 128, any k they divide: 1 byte a row and k-step (a word in LDS)
-       MX_SCALES_ANY = 4 };      // blocks of 32, k no multiple of 128: 1 byte a row and block, likewise (16 words a row: no room beside 256 x 256 tiles)
-
 // What the k-steps of the last round past the end of k multiply by: zero codes (a round is four k-steps whatever k is; the loop body then
 // has no branch, which its 256 accumulators would not survive in registers).
 static __device__ const u4v tf_mx_zeros[64] = {};
-
-// The largest tiles of a product of E2M1 rows: several a workgroup, one after the other, the next one's first k-steps on their way while the
-// last one's results are formed (16,384 x 4,096 x 2,048: 106 -> 87 us, 16,384 x 8,192 x 4,096: 314 -> 294).  E4M3 rows' operands leave too few registers
-// for it (4,096 x 4,096 x 4,096: 55 -> 57 us, 16,384 x 8,192 x 4,096: 486 -> 473), and a gated product's results spill beside them (16,384 x 8,192 x
-// 4,096: 945 -> 1,140).
-constexpr bool tf_mx_persistent(bool fp4_rows, bool gated, int products) { return fp4_rows && !gated && products == 64; }
 
 // LDS of a workgroup: the ring, the weights' scales of a round, the rows' (a word a row and block where SC is MX_SCALES_ANY).
 constexpr int tf_mx_scale_rows(int fm, int wm) { return 16 * fm * wm < 64 ? 64 : 16 * fm * wm; }
@@ -450,69 +437,46 @@ inline int tf_mx_gemm_tiles(const MxArgs& p, int cus, hipStream_t s) {
     tf_mx_gemm<FP4A, GATED, SC, FM, FT, WM, WN, NS><<<(unsigned)grid, 256, 0, s>>>(p, tiles_m, tiles_n);
     return (int)hipGetLastError();
 }
-// The tile's size.  A 256 x 256 tile takes 54 us of a CU at k = 4,096 (E4M3 rows), one of 128 x 128 (two a CU at once) 14.5 us, one of 64 x 64
-// 6 us (plus 3 us once): the large ones read LDS and L2 least for a product, the small ones give every CU something to do.
-//  - 32 x 64 while they are at most one a CU: 64 rows x 4,096: 6.8 us against 7.4 of 64 x 64, 64 rows x 8,192 x 8,192: 13.1, 15.1; 256 rows (two a CU): 9.4, 8.3
-//  - 64 x 64 while they are at most two a CU: 256 rows x 4,096: 8.5 us, against 14.8 (128) and 40 (256); 512 rows: 13.6, 15.8, 41
-//  - 256 x 256 where whole rounds of them cost less than whole rounds of 128 x 128, a quarter of the work at 15 / 16 of the time: 4,096 rows x
-//    4,096: 54 us against 58; but 2,048 rows (half the CUs without a tile) 46 against 30, 16 x 18 tiles (two rounds for 1.1) 74 against 70
-//  - else 128 x 128: 1,024 rows: 18.8 us, against 25.5 (64) and 42 (256)
-// All of these were taken with E4M3 rows at a k of 4,096; the rule stands unmeasured for E2M1 rows, gated products and other k.  It is known to be off where k is no
-// multiple of 128 with blocks of 32: no 256 x 256 tile has room for the scales, and of E4M3 rows' 128 x 128 one fits a CU instead of two (4,096 x
-// 4,096 x 4,128 88 us, x 4,224 57; E2M1 rows 62 and the gated 4,096 x 2,048 x 4,128 94).
-// Blocks of 128 columns of a gated product's codes need the tile's columns to be whole blocks: 64 rows x 128 columns in place of the two
-// smaller ones, or, where 64 x 64 would be chosen and the activation goes to memory too, its codes in a launch of their own behind those
-// (64 rows x 2,048 x 4,096: 15.2 -> 9.0 us).
-inline int tf_mx_tile_size(const MxArgs& p, bool fp4_rows, bool gated, int cus) {
-    auto tiles = [&](int rows, int cols) { return (long long)((p.rows + rows - 1) / rows) * ((p.n * (gated ? 2ll : 1ll) + cols - 1) / cols); };
-    auto rounds = [&](long long t) { return (t + cus - 1) / cus; };
-    if (tiles(32, 64) <= cus) return -1;
-    if (tiles(64, 64) <= 2 * cus) return 0;
-    // the persistent workgroups store whole 16-byte pieces, at 31-bit offsets from the tile's first row
-    if (tf_mx_persistent(fp4_rows, gated, 64) && (p.wide != 2 || p.n % 8 != 0 || p.out_stride > (1 << 21))) return 1;
-    return 15 * rounds(tiles(256, 256)) <= 4 * rounds(tiles(128, 128)) ? 2 : 1;
-}
 template <bool FP4A, bool GATED, int SC>
-inline int tf_mx_gemm_small(const MxArgs& p, int size, int cus, hipStream_t s) {
-    return size < 0 ? tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 2, 2, 2, 4>(p, cus, s) : tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, cus, s);
-}
-template <bool FP4A, bool GATED, int SC>
-inline int tf_mx_gemm_go(const MxArgs& p, int cus, hipStream_t s) {
-    const int size = tf_mx_tile_size(p, FP4A, GATED, cus);
-    if constexpr (SC != MX_SCALES_ANY)
-        if (size == 2) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, FP4A ? 4 : 3>(p, cus, s);
-    if constexpr (GATED)
-        if (p.codes != nullptr && p.out_block == 128) {
-            if (size <= 0 && p.act != nullptr) {
-                MxArgs first = p;
-                first.codes = first.scales = nullptr;
-                const int status = tf_mx_gemm_small<FP4A, GATED, SC>(first, size, cus, s);
-                return status ? status : tf_launch_mx_codes(p, s);
-            }
-            return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, FP4A ? 4 : 3>(p, cus, s);
-        }
-    if (size >= 1) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, FP4A ? 4 : 3>(p, cus, s);
-    return tf_mx_gemm_small<FP4A, GATED, SC>(p, size, cus, s);
-}
-template <bool FP4A, bool GATED>
-inline int tf_launch_mx_gemm(const MxArgs& p, int cus, hipStream_t s) {
-    const size_t at = (size_t)p.a_scales;
-    if (p.block_shift == 5) {
-        if (p.k % 512 == 0 && at % 16 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_32>(p, cus, s);
-        if (p.k % 128 == 0 && at % 4 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_STEP_32>(p, cus, s);
-        return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_ANY>(p, cus, s);
-    }
-    if constexpr (!FP4A) {
-        if (p.k % 512 == 0 && at % 4 == 0) return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_128>(p, cus, s);
-        return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_STEP_128>(p, cus, s);
+inline int tf_mx_gemm_go(const MxArgs& p, int tile, int cus, hipStream_t s) {
+    constexpr int STAGES = FP4A ? 4 : 3;
+    switch (tile) {
+    case MX_TILE_32X64: return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 2, 2, 2, 4>(p, cus, s);
+    case MX_TILE_64X64: return tf_mx_gemm_tiles<FP4A, GATED, SC, 1, 4, 4, 1, 4>(p, cus, s);
+    case MX_TILE_128X128: return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 2, 2, STAGES>(p, cus, s);
+    case MX_TILE_256X256:
+        if constexpr (SC != MX_SCALES_ANY) return tf_mx_gemm_tiles<FP4A, GATED, SC, 8, 8, 2, 2, STAGES>(p, cus, s);
+        break;
+    case MX_TILE_64X256:                                                     // (a context has one width of MXFP8 blocks: E4M3 rows of 32 have codes of 32)
+        if constexpr (GATED && (FP4A || SC == MX_SCALES_128 || SC == MX_SCALES_STEP_128)) return tf_mx_gemm_tiles<FP4A, GATED, SC, 4, 4, 1, 4, STAGES>(p, cus, s);
+        break;
     }
     return -1;
 }
-// Both regimes of the products.  The streaming kernel reads every weight once for all its rows, but each workgroup reads all the rows: it takes
-// up to 32 (4,096 x 4,096: 24 rows 5.2 us against 6.7 of the tiles, 40 rows 7.9 against 6.7), and 16 of a gated product, which has twice
-// the weights a column (2,048 x 4,096: 16 rows 6.2 us against 7.2, 24 rows 8.3 against 7.2).
+template <bool FP4A, bool GATED>
+inline int tf_mx_gemm_launch(const MxArgs& p, const MxChoice& choice, int cus, hipStream_t s) {
+    switch (choice.scales) {
+    case MX_SCALES_32: return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_32>(p, choice.kernel, cus, s);
+    case MX_SCALES_STEP_32: return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_STEP_32>(p, choice.kernel, cus, s);
+    case MX_SCALES_ANY: return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_ANY>(p, choice.kernel, cus, s);
+    }
+    if constexpr (!FP4A)
+        switch (choice.scales) {
+        case MX_SCALES_128: return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_128>(p, choice.kernel, cus, s);
+        case MX_SCALES_STEP_128: return tf_mx_gemm_go<FP4A, GATED, MX_SCALES_STEP_128>(p, choice.kernel, cus, s);
+        }
+    return -1;
+}
+template <bool FP4A, bool GATED>
+inline int tf_mx_launch(const MxArgs& p, const MxChoice& choice, int cus, hipStream_t s) {
+    return choice.kernel <= MX_FEW_128 ? tf_mx_stream_launch<FP4A, GATED>(p, choice.kernel, s) : tf_mx_gemm_launch<FP4A, GATED>(p, choice, cus, s);
+}
 inline int tf_launch_mx(const MxArgs& p, bool gated, bool fp4_rows, int cus, hipStream_t s) {
-    if (p.rows <= (gated ? 16 : 32)) return fp4_rows ? tf_launch_mx_stream<true>(p, gated, cus, s) : tf_launch_mx_stream<false>(p, gated, cus, s);
-    if (gated) return fp4_rows ? tf_launch_mx_gemm<true, true>(p, cus, s) : tf_launch_mx_gemm<false, true>(p, cus, s);
-    return fp4_rows ? tf_launch_mx_gemm<true, false>(p, cus, s) : tf_launch_mx_gemm<false, false>(p, cus, s);
+    const MxChoice choice = tf_mx_choose({p.rows, p.n, p.k, cus, fp4_rows, gated, p.block_shift, (size_t)p.a_scales, p.wide, p.out_stride, p.act != nullptr,
+                                          p.codes != nullptr, p.out_block});
+    MxArgs first = p;
+    if (choice.codes_apart) first.codes = first.scales = nullptr;
+    const int status = gated ? fp4_rows ? tf_mx_launch<true, true>(first, choice, cus, s) : tf_mx_launch<false, true>(first, choice, cus, s)
+                             : fp4_rows ? tf_mx_launch<true, false>(first, choice, cus, s) : tf_mx_launch<false, false>(first, choice, cus, s);
+    return status || !choice.codes_apart ? status : tf_launch_mx_codes(p, s);
 }

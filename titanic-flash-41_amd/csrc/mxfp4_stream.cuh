@@ -5,6 +5,7 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 weight rows (first operand) and 16 token rows over 128 columns; both formats
 // are decoded and both scales applied in the matrix core, sums are FP32.
 #pragma once
+#include "mxfp4_choice.hpp"
 #include "mxfp4_codec.cuh"
 #include <type_traits>
 
@@ -276,23 +277,13 @@ inline int tf_launch_mx_codes(const MxArgs& p, hipStream_t s) {
     tf_mx_codes<<<(items + 255) / 256, 256, 0, s>>>(p, items);
     return (int)hipGetLastError();
 }
-// Few rows.  A workgroup fills a CU.  Columns a workgroup: 16 while that is one round of workgroups (4 rows x 4,096 x 4,096: 3.6 us against 4.0 of 32
-// columns), else 32 (16 rows x 5,120 x 4,096: 4.4 against 6.6, 32 rows x 8,192 x 8,192: 10.2 against 15.3).  A gated product's hold whole
-// blocks of its codes: 32, or 128 of blocks of 128 where the activation itself has nowhere to go.  With the activation in memory those codes
-// are a launch of their own behind 16 columns a workgroup (4 rows x 2,048 x 4,096: 16 workgroups 11.8 us, 128 and the second launch 7.2).
-template <bool FP4A>
-inline int tf_launch_mx_stream(const MxArgs& p, bool gated, int cus, hipStream_t s) {
-    const bool wide = (p.n + 15) / 16 > cus;
-    if (!gated) {
-        if (p.rows <= 16) return wide ? tf_mx_stream_go<FP4A, false, 2, 1, 1, 16>(p, s) : tf_mx_stream_go<FP4A, false, 1, 1, 1, 16>(p, s);
-        return wide ? tf_mx_stream_go<FP4A, false, 2, 2, 1, 8>(p, s) : tf_mx_stream_go<FP4A, false, 1, 2, 1, 8>(p, s);
+template <bool FP4A, bool GATED>
+inline int tf_mx_stream_launch(const MxArgs& p, int kernel, hipStream_t s) {
+    if constexpr (GATED) {
+        if (kernel == MX_FEW_128) return tf_mx_stream_go<FP4A, true, 2, 1, 4, 16>(p, s);
+        return kernel == MX_FEW_32 ? tf_mx_stream_go<FP4A, true, 2, 1, 1, 16>(p, s) : tf_mx_stream_go<FP4A, true, 1, 1, 1, 16>(p, s);
+    } else {
+        if (p.rows <= 16) return kernel == MX_FEW_32 ? tf_mx_stream_go<FP4A, false, 2, 1, 1, 16>(p, s) : tf_mx_stream_go<FP4A, false, 1, 1, 1, 16>(p, s);
+        return kernel == MX_FEW_32 ? tf_mx_stream_go<FP4A, false, 2, 2, 1, 8>(p, s) : tf_mx_stream_go<FP4A, false, 1, 2, 1, 8>(p, s);
     }
-    if (p.codes == nullptr || (p.out_block == 128 && p.act != nullptr)) {
-        MxArgs first = p;
-        first.codes = first.scales = nullptr;
-        const int status = wide ? tf_mx_stream_go<FP4A, true, 2, 1, 1, 16>(first, s) : tf_mx_stream_go<FP4A, true, 1, 1, 1, 16>(first, s);
-        return status || p.codes == nullptr ? status : tf_launch_mx_codes(p, s);
-    }
-    if (p.out_block == 128) return tf_mx_stream_go<FP4A, true, 2, 1, 4, 16>(p, s);
-    return tf_mx_stream_go<FP4A, true, 2, 1, 1, 16>(p, s);
 }
