@@ -111,9 +111,10 @@ int ca_ffn_add_norm_quant(void* context, int rows, int cols, const void* x, int6
                           const void* weight, float eps, void* residual_out, int64_t residual_out_stride, void* normed, void* codes, void* scales,
                           void* codes_min, void* scales_min, void* stream);
 /* x [rows][cols] of CA_TYPE_* -> words and scales, in the canonical layout that ca_mxfp4_prepare and the expert preparation take.  A
- * block's scale byte is floor(log2(amax)) - 2 + 127 within 1..247 (127 for a zero block), codes round to the nearest, ties to
- * even, and saturate; a block that holds a NaN or an infinity has scale byte 255 and reads back as NaN.  cols: a multiple of 32;
- * rows start at 16-byte boundaries; rows * cols < 2^34. */
+ * block's scale byte is floor(log2(amax)) - 2 + 127 within 1..247, codes round to the nearest, ties to even, and saturate (which
+ * the bound of 247 makes of blocks past 2^123: their largest code stands for 6 * 2^120); a block whose amax is zero or subnormal in
+ * FP32, below 2^-126, is a zero block, with scale byte 127 and zero codes; one that holds a NaN or an infinity has scale byte 255
+ * and reads back as NaN.  cols: a multiple of 32; rows start at 16-byte boundaries; rows * cols < 2^34. */
 int ca_mxfp4_quant(void* context, int rows, int cols, const void* x, int64_t x_stride, int x_type, void* words, void* scales, void* stream);
 /* The values that words and scales stand for, rounded once to out_type. */
 int ca_mxfp4_dequant(void* context, int rows, int cols, const void* words, const void* scales, void* out, int64_t out_stride, int out_type, void* stream);

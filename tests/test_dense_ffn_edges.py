@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from helpers import native
-from test_dense_ffn import Gpu, f64, fake_context, norm_want, normal, quant8
+from helpers import native, synth
+from test_dense_ffn import Gpu, f64, fake_context, norm_want, normal, quant8, values4
 
 
 @pytest.fixture(scope="module")
@@ -84,3 +84,25 @@ def test_norm_of_rows_that_are_not_finite(gpu, rows, cols):
     keep = [i for i in range(rows) if i not in (2, 4, 6)]
     assert all(torch.equal(a[keep], b[keep]) for a, b in zip(clean[:4], (r, n, c, s)))
     assert bool(torch.isnan(n[2]).all()) and bool(torch.isnan(n[4, 3])) and bool(torch.isinf(r[6, 9])) and bool(torch.isnan(n[6, 9]))
+
+
+# ---- the ends of the quantizer's range ----------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_blocks_at_the_ends_of_the_range(gpu, dtype):
+    """As the header has it, and the generator of the experts' weights: a block below 2^-126 is a zero block, one past 2^123 saturates."""
+    g = gpu(32)
+    largest = [2.0 ** -133, 2.0 ** -128, 2.0 ** -127, 2.0 ** -126 * (1 - 2.0 ** -7), 2.0 ** -126, 2.0 ** -125, 2.0 ** -124, 2.0 ** 122 * 1.75, 2.0 ** 123, 2.0 ** 127 * 1.5]
+    x = torch.zeros(len(largest), 32, dtype=torch.float64)
+    x[:, 3] = torch.tensor(largest, dtype=torch.float64)
+    x[:, 20], x[:, 21] = -x[:, 3], x[:, 3] / 2
+    x = x.to(dtype)
+    words, scales = g.quant(x.cuda())
+    assert scales.flatten().tolist() == [127, 127, 127, 127, 1, 1, 1, 247, 247, 247]
+    back = f64(g.dequant(words, scales, 2))
+    assert not back[:4].any()
+    assert back[4:7, 3].tolist() == largest[4:7]
+    assert np.array_equal(back[7:, 3], [6 * 2.0 ** 120] * 3) and np.array_equal(back[:, 20], -back[:, 3])
+    generated = synth.quantize_mxfp4(x.float())                      # (whose zero blocks keep the signs of their zeros)
+    assert np.array_equal(values4(words, scales), values4(*generated)) and torch.equal(scales.cpu(), generated[1]) and not bool(words[:4].any())
