@@ -96,7 +96,10 @@ int ca_ffn_sum_residual(void* context, int rows, int live, const void* routes, c
  * argument.  All calls: rows 0 enqueues nothing and returns 0; -1 for a null or misaligned pointer, a size outside the
  * ranges below, a stride shorter than its row, or a context opened on another device than the current one; nothing is
  * allocated, kept from one call for the next, or waited for, so calls may overlap on any streams and be captured.  No output
- * overlaps an input or another output unless it says so.  rows <= 4,194,304 except in the two quantizers. */
+ * overlaps an input or another output unless it says so.  rows <= 4,194,304 except in the two quantizers.  The same call gives the
+ * same bits every time.  The norm and both products sum in an order that depends on the sizes, the number of rows among them: a row's
+ * values may differ by a rounding of their last bit (and its codes and scales by what follows from that) between calls of different
+ * row counts; what the quantizers make of a row, and the norm's residual, do not. */
 #define CA_TYPE_BF16 0
 #define CA_TYPE_FP16 1
 #define CA_TYPE_FP32 2

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from helpers import native, synth
-from test_dense_ffn import Gpu, f64, fake_context, norm_want, normal, quant8, values4
+from test_dense_ffn import Gpu, activations, f64, fake_context, mxfp4, norm_want, normal, product_error, quant8, swiglu_want, values4
 
 
 @pytest.fixture(scope="module")
@@ -106,3 +106,41 @@ def test_blocks_at_the_ends_of_the_range(gpu, dtype):
     assert np.array_equal(back[7:, 3], [6 * 2.0 ** 120] * 3) and np.array_equal(back[:, 20], -back[:, 3])
     generated = synth.quantize_mxfp4(x.float())                      # (whose zero blocks keep the signs of their zeros)
     assert np.array_equal(values4(words, scales), values4(*generated)) and torch.equal(scales.cpu(), generated[1]) and not bool(words[:4].any())
+
+
+# ---- a row in calls of different row counts ------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [384, 1024, 2048, 4096, 8192])
+def test_a_row_alone_and_among_many(gpu, cols):
+    """Few rows and many are summed in different orders, so a row's BF16 values may differ by a rounding (never its residual): each is within half a
+    step and the chain of the formula's, so they are within two of that of each other."""
+    g = gpu(32)
+    rows = 600
+    x, res = normal("edges/x", rows, cols).to(torch.bfloat16).cuda(), normal("edges/r", rows, cols).to(torch.bfloat16).cuda()
+    w = (1.0 + normal("edges/norm-w", cols, std=0.2)).to(torch.bfloat16).cuda()
+    many = g.norm(x, res, w, minimum=False)
+    for at in (0, 7, rows - 1):
+        one = g.norm(x[at:at + 1], res[at:at + 1], w, minimum=False)
+        assert torch.equal(one[0][0], many[0][at])
+        a, b = f64(one[1][0]), f64(many[1][at])
+        assert np.all(np.abs(a - b) <= np.abs(b) * (1 + 2.0 ** -7) * 2 * (2.0 ** -8 + 48 * 2.0 ** -24)) and np.mean(a != b) < 1e-2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,block", [(0, 32), (0, 128), (1, 32)])
+def test_a_token_in_a_small_and_a_large_batch(gpu, kind, block):
+    """The same row through every regime of the products: the streaming kernels, and each size of tile."""
+    g = gpu(block)
+    n, k = 1152, 1664
+    a, a_scales, av = activations(g, kind, 4500, k, std=2.0)
+    ups, gates = mxfp4("up", n, k, std=0.1), mxfp4("gate", n, k, std=0.1)
+    up, gate = g.prepare(*ups), g.prepare(*gates)
+    uv, gv = values4(*ups), values4(*gates)
+    want, bound = av[:4] @ uv.T, product_error(av[:4], uv, kind)
+    h_want, h_bound = swiglu_want(av[:4], uv, gv, kind)
+    for rows in (4, 16, 30, 60, 400, 1100, 4500):
+        out = f64(g.linear(rows, n, k, a[:rows], a_scales[:rows], kind, up)[:4])
+        assert np.all(np.abs(out - want) <= np.abs(want) * 2.0 ** -8 + bound), rows
+        h = f64(g.swiglu(rows, n, k, a[:rows], a_scales[:rows], kind, up, gate)[0][:4])
+        assert np.all(np.abs(h - h_want) <= np.abs(h_want) * 2.0 ** -8 + h_bound), rows
