@@ -123,7 +123,8 @@ int ca_mxfp4_quant(void* context, int rows, int cols, const void* x, int64_t x_s
 int ca_mxfp4_dequant(void* context, int rows, int cols, const void* words, const void* scales, void* out, int64_t out_stride, int out_type, void* stream);
 /* Weights [n][k] from the canonical layout to the one that the products read (once, at load time; the layout of the layer's prepared
  * experts, padded with zeros to whole tiles): bytes of the two destinations, and the copy.  n from 1 to 2^24, k a multiple of 32
- * up to 65,536, n * k up to 2^36, here and in both products. */
+ * up to 65,536, n * k up to 2^36, here and in both products; words and both destinations 16-byte aligned, here and there.  (The
+ * products also refuse, with -1, a launch of 2^32 threads or more: none up to rows * n = 2^36 is.) */
 int64_t ca_mxfp4_words_bytes(int n, int k);
 int64_t ca_mxfp4_scales_bytes(int n, int k);
 int ca_mxfp4_prepare(void* context, int n, int k, const void* words, const void* scales, void* prepared_words, void* prepared_scales, void* stream);
