@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_qua
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int row = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     if (row >= p.rows) return;                             // a whole wave (WAVES 1: no barrier below) or nobody
-    const int t = WAVES == 1 ? lane : threadIdx.x, per_row = p.cols >> 3, group_lanes = p.act_block >> 3;
+    const int t = WAVES == 1 ? lane : threadIdx.x, per_row = p.cols >> 3, group_bits = p.act_block == 128 ? 4 : 2, group_lanes = 1 << group_bits;
     const u4v* x = reinterpret_cast<const u4v*>(p.x + (long long)row * p.x_stride);
     const u4v* res = reinterpret_cast<const u4v*>(p.residual + (long long)row * p.residual_stride);
     const u4v* weight = reinterpret_cast<const u4v*>(p.weight);
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_qua
     // Squares of BF16 values reach 2^256 and 2^-266.  Where their sum passes FP32's range, or is so small that squares of the row vanished in it, the
     // row's statistics are formed again with the row scaled by a power of two: 2^-80 (its largest square is then 2^96) or 2^80 (the
     // sum was below 2^-83, so the largest is 2^77, the least 2^-106).  1 / root is as small as 2^-128 for large rows, a subnormal: 2^8 of it goes to the row.
-    if (!(mean >= 0x1p-96f && mean < __builtin_inff())) {      // the whole row's lanes alike; NaN too, and comes out as NaN
+    if (__builtin_expect(!(mean >= 0x1p-96f && mean < __builtin_inff()), 0)) {      // the whole row's lanes alike; NaN too, and comes out as NaN
         const bool small = mean < 1.f;
         const float scale = small ? 0x1p80f : 0x1p-80f, share = small ? 0x1p80f : 0x1p-8f;
         ss = 0.f;
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_qua
         inverse = 1.0f / __builtin_sqrtf(__fadd_rn(ss / (float)p.cols, __fmul_rn(__fmul_rn(p.eps, scale), scale)));
         if (!small) inverse = __fmul_rn(inverse, 0x1p-72f);
     }
-    const int groups = p.cols / p.act_block;
+    const int groups = per_row >> group_bits;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int q = i * LANES + t;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_qua
         const float amax = tf_group_amax(v, group_lanes);
         if (!on) continue;
         const size_t at = (size_t)row * per_row + q;
-        const size_t group = (size_t)row * groups + q / group_lanes;
+        const size_t group = (size_t)row * groups + (q >> group_bits);
         if (p.normed != nullptr) reinterpret_cast<u4v*>(p.normed)[at] = o;
         if (p.codes != nullptr) {
             const Quant8 c = tf_quant8(v, amax, 0.f);
