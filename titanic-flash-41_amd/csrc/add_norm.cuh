@@ -125,9 +125,9 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) tf_add_norm_qua
     }
 }
 // Up to two rows a CU the latency of the row's own loads, sums and exchange is the time, so a lane takes one piece (4 rows x 1,024: 2.7 us against 3.3
-// of one wave with two pieces, x 4,096: 2.95 against 3.5 of four waves, x 8,192: 4.6 against 5.8; 512 rows x 4,096: 5.5 against 5.9).  Beyond, HBM
+// of one wave with two pieces, x 4,096: 2.9 against 3.5 of four waves, x 8,192: 4.6 against 5.8; 512 rows x 4,096: 5.5 against 5.9).  Beyond, HBM
 // is: fewer waves that meet at a barrier and more loads in flight a lane (2,048 rows x 4,096: 14.2 of eight waves against 13.1, 16,384 x 5,120: 144
-// against 134 us = 5.65 TB/s of the 9 bytes a value that the row moves; 16,384 x 1,024: four waves 28, one 23.5; 16,384 x 4,096 with a wave a row
+// against 132 us = 5.7 TB/s of the 9 bytes a value that the row moves; 16,384 x 1,024: four waves 28, one 23.5; 16,384 x 4,096 with a wave a row
 // 117 against 106).  The order of the sum of squares follows the variant.
 inline void tf_launch_add_norm(const AddNormArgs& p, int cus, hipStream_t s) {
     const int quarter = (p.rows + 3) / 4;
