@@ -144,3 +144,47 @@ def test_a_token_in_a_small_and_a_large_batch(gpu, kind, block):
         assert np.all(np.abs(out - want) <= np.abs(want) * 2.0 ** -8 + bound), rows
         h = f64(g.swiglu(rows, n, k, a[:rows], a_scales[:rows], kind, up, gate)[0][:4])
         assert np.all(np.abs(h - h_want) <= np.abs(h_want) * 2.0 ** -8 + h_bound), rows
+
+
+# ---- captured, beside other work ---------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_two_launches_and_persistent_workgroups_captured_beside_each_other(gpu):
+    """A gated product whose codes are a launch of their own, and a product of several tiles a workgroup, in graphs on two streams that run at once: every
+    replay gives the eager bits of its new rows."""
+    g, p = gpu(128), native.ptr
+    n, k, rows, wide, many = 1152, 640, 60, 4088, 8190
+    up, gate = g.prepare(*mxfp4("up", n, k, std=0.1)), g.prepare(*mxfp4("gate", n, k, std=0.1))
+    w = g.prepare(*mxfp4("w", wide, 512))
+    a, a_scales, _ = activations(g, 0, rows, k, std=2.0)
+    b, b_scales, _ = activations(g, 1, many, 512)
+    e = lambda *shape, dtype=torch.uint8: torch.empty(shape, dtype=dtype, device="cuda")
+    sets = [(e(rows, n, dtype=torch.bfloat16), e(rows, n), e(rows, n // 128), e(many, wide, dtype=torch.bfloat16)) for _ in range(2)]
+
+    def gated(out):
+        assert g.lib.ca_mxfp4_swiglu(g.ctx, rows, n, k, p(a), p(a_scales), 0, p(up[0]), p(up[1]), p(gate[0]), p(gate[1]), p(out[0]), p(out[1]), p(out[2]), 0, g.stream()) == 0
+
+    def product(out):
+        assert g.lib.ca_mxfp4_linear(g.ctx, many, wide, 512, p(b), p(b_scales), 1, p(w[0]), p(w[1]), p(out[3]), wide, g.stream()) == 0
+
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    torch.cuda.synchronize()
+    for call, stream, graph in zip((gated, product), streams, graphs):
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(3):
+                call(sets[0])
+    for i in range(4):
+        a.copy_(a.roll(7 * i + 1, 0).clone())
+        b.copy_(b.roll(13 * i + 1, 0).clone())
+        for t in sets[0]:
+            t.view(torch.uint8).fill_(0x11)
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        gated(sets[1])
+        product(sets[1])
+        torch.cuda.synchronize()
+        for got, want in zip(*sets):
+            assert torch.equal(got.view(torch.uint8), want.view(torch.uint8)), i
